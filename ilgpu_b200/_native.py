@@ -18,7 +18,7 @@ LIB_PATH = os.environ.get("B200ALG_LIBRARY") or os.path.join(_HERE, "libb200alg.
 OK, INVALID_ARGUMENT, UNSUPPORTED, TEMP_TOO_SMALL, CUDA_ERROR, WAIT_LIMIT, MISALIGNED, TOO_LARGE, STATIC_LIMIT = range(9)
 
 # dtype codes
-I8, U8, I16, U16, I32, U32, I64, U64, F16, F32, F64 = range(11)
+I8, U8, I16, U16, I32, U32, I64, U64, F16, F32, F64, BF16 = range(12)
 ADD, MAX, MIN = range(3)
 SORT_ASCENDING, SORT_DESCENDING, SORT_FLOAT_TOTAL_ORDER = 0, 1, 2
 LOCATOR_EQUAL_WIDTH_CLAMP, LOCATOR_MODULO = 0, 1
@@ -54,6 +54,16 @@ SIGNATURES = {
     "b200alg_unique_to_host": (_int, [_vp, _vp, _i64, _int, _vp, _vp, _i64]),
     "b200alg_run_length_encode_temp_bytes": (_int, [_int, _i64, ctypes.POINTER(_i64)]),
     "b200alg_run_length_encode": (_int, [_vp, _vp, _i64, _int, _vp, _vp, _vp, _vp, _i64]),
+    "b200alg_embedding": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _i64, _int, _dbl, _vp, _i64, _int]),
+    "b200alg_embedding_gradient_temp_bytes": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "b200alg_embedding_gradient": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _i64, _int, _dbl, _vp, _i64, _i64, _i64, _int, _int, _vp, _i64]),
+    "b200alg_gradient_norm_temp_bytes": (_int, [_i64, ctypes.POINTER(_i64)]),
+    "b200alg_gradient_norm": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64]),
+    "b200alg_gradient_scale": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _dbl]),
+    "b200alg_gradient_clip": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _dbl, _vp, _vp, _i64]),
+    "b200alg_balance_loss_temp_bytes": (_int, [_i64, _i64, ctypes.POINTER(_i64)]),
+    "b200alg_balance_loss": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _i64, _int, _vp, _dbl, _vp, _vp, _vp, _vp, _i64]),
+    "b200alg_balance_loss_gradient": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _i64, _dbl, _vp, _vp, _i64, _int]),
     "b200alg_device_status": (_int, [_vp, _vp]),
 }
 

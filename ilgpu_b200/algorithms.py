@@ -14,6 +14,12 @@ source tree, ``Src/ILGPU.Algorithms``):
 * operation types ``Add/Max/Min{Int32,Int64,UInt32,UInt64,Float,Double}`` -
   ScanReduceOperations.tt:20-74; ``Ascending*/Descending*`` - RadixSortOperations.tt:26-125
 
+Beside them, in the same manner and without a counterpart in the reference, the operators of a
+language model's training step that are built from these primitives: ``CreateEmbedding`` and
+``CreateEmbeddingGradient`` (sorted pairs), ``CreateGradientNorm``, ``CreateGradientClip`` and
+``CreateGradientScale`` (reduction), ``CreateBalanceLoss`` and ``CreateBalanceLossGradient``
+(histogram).  Their matrices are two-dimensional tensors with dense rows.
+
 An ``ArrayView1D<T, TStride>`` is a one-dimensional ``torch`` CUDA tensor (its stride is
 the view's stride; dense = 1); ``ArrayView<int>`` temp views are int32 tensors.  A stream
 argument is a ``torch.cuda.Stream`` or ``None`` (= the current stream).  PyTorch only
@@ -77,6 +83,8 @@ _TORCH_TO_CODE = {
     torch.int32: N.I32, torch.uint32: N.U32, torch.int64: N.I64, torch.uint64: N.U64,
     torch.float16: N.F16, torch.float32: N.F32, torch.float64: N.F64,
 }
+# element types of the operators of a training step
+_ELEMENT_TO_CODE = {torch.float16: N.F16, torch.float32: N.F32, torch.bfloat16: N.BF16}
 _TYPE_NAMES = {
     "Int8": torch.int8, "UInt8": torch.uint8, "Int16": torch.int16, "UInt16": torch.uint16,
     "Int32": torch.int32, "UInt32": torch.uint32, "Int64": torch.int64, "UInt64": torch.uint64,
@@ -193,6 +201,74 @@ def _check_view(view, name: str, dtype: torch.dtype | None = None) -> None:
         raise InvalidOperationException(f"{name}: element type {view.dtype}, expected {dtype}")
     if view.numel() > 1 and view.stride(0) < 1:
         raise ArgumentOutOfRangeException(f"{name}: stride")
+
+
+def _element_code(view: torch.Tensor, name: str) -> int:
+    try:
+        return _ELEMENT_TO_CODE[view.dtype]
+    except KeyError:
+        raise NotSupportedException(f"{name}: element type {view.dtype}") from None
+
+
+def _check_matrix(view, name: str, width: int | None = None) -> None:
+    if view is None or not isinstance(view, torch.Tensor):
+        raise ArgumentNullException(name)
+    if view.dim() != 2:
+        raise ArgumentOutOfRangeException(f"{name}: two-dimensional view expected")
+    if not view.is_cuda:
+        raise InvalidOperationException(f"{name}: the view is not in CUDA device memory")
+    if view.size(1) > 1 and view.stride(1) != 1:
+        raise NotSupportedException(f"{name}: the rows of a matrix are dense")
+    if view.size(0) > 1 and view.stride(0) < view.size(1):
+        raise ArgumentOutOfRangeException(f"{name}: stride")
+    if width is not None and view.size(1) != width:
+        raise ArgumentOutOfRangeException(f"{name}: {view.size(1)} columns, expected {width}")
+
+
+def _check_index_type(view, name: str) -> None:
+    if view.dtype not in (torch.int32, torch.int64):
+        raise NotSupportedException(f"{name}: element type {view.dtype}, expected int32 or int64")
+
+
+def _row_stride(view: torch.Tensor) -> int:
+    return view.stride(0) if view.size(0) > 1 else view.size(1)
+
+
+def _check_element(view, name: str, dtype: torch.dtype = torch.float32, length: int = 1) -> None:
+    _check_view(view, name, dtype)
+    if view.numel() < length:
+        raise ArgumentOutOfRangeException(name)
+    if length > 1 and _stride(view) != 1:
+        raise NotSupportedException(f"{name}: dense view expected")
+
+
+def _check_views(views, name: str) -> None:
+    if views is None or not isinstance(views, (list, tuple)):
+        raise ArgumentNullException(name)
+    for i, view in enumerate(views):
+        if view is None or not isinstance(view, torch.Tensor):
+            raise ArgumentNullException(f"{name}[{i}]")
+        if not view.is_cuda:
+            raise InvalidOperationException(f"{name}[{i}]: the view is not in CUDA device memory")
+        if not view.is_contiguous():
+            raise NotSupportedException(f"{name}[{i}]: dense view expected")
+        _element_code(view, f"{name}[{i}]")
+
+
+def _check_mask(mask, tokens: int) -> None:
+    if mask is None:
+        return
+    _check_view(mask, "mask")
+    if mask.dtype not in (torch.bool, torch.uint8):
+        raise InvalidOperationException(f"mask: element type {mask.dtype}, expected bool or uint8")
+    if mask.numel() < tokens:
+        raise ArgumentOutOfRangeException("mask")
+    if _stride(mask) != 1:
+        raise NotSupportedException("mask: dense view expected")
+
+
+def _array(kind, values):
+    return (kind * len(values))(*values)
 
 
 def _stride(view: torch.Tensor) -> int:
@@ -586,6 +662,206 @@ class Accelerator:
         with self.Bind():
             B200AlgException.ThrowIfFailed(self.L.b200alg_sequence(
                 _stream_ptr(stream), _ptr(view), view.numel(), dtype_code(view.dtype), int(start), int(step)))
+
+    # -- operators of a training step: embedding --
+    def _check_device(self, *views) -> None:
+        device = torch.device("cuda", torch.cuda.current_device()) if self.device.index is None else self.device
+        for view in views:
+            if view is not None and view.device != device:
+                raise InvalidOperationException(f"a view on {view.device}, expected {device}")
+
+    def CreateEmbedding(self):
+        """Returns ``embed(stream, table, tokens, output, scale=1.0)``: ``output[i, :] = scale *
+        table[tokens[i], :]``, zeros for a token outside the table.  Tokens are int32 or int64; table and
+        output are float32, float16 or bfloat16, not necessarily the same.  Rows of ``output`` behind the
+        last token are left alone."""
+        fast, index = self._host.embedding, self._index
+
+        def embed(stream, table, tokens, output, scale=1.0):
+            if fast(index, stream, table, tokens, output, scale):
+                return
+            _check_matrix(table, "table")
+            _check_view(tokens, "tokens")
+            _check_matrix(output, "output", table.size(1))
+            _check_index_type(tokens, "tokens")
+            types = _element_code(table, "table"), _element_code(output, "output")
+            if output.size(0) < tokens.numel():
+                raise ArgumentOutOfRangeException("output")
+            self._check_device(table, tokens, output)
+            with self.Bind():
+                B200AlgException.ThrowIfFailed(self.L.b200alg_embedding(
+                    _stream_ptr(stream), _ptr(table), table.size(0), table.size(1), _row_stride(table), types[0], _ptr(tokens), tokens.numel(),
+                    _stride(tokens), dtype_code(tokens.dtype), float(scale), _ptr(output), _row_stride(output), types[1]))
+
+        return embed
+
+    def ComputeEmbeddingGradientTempStorageSize(self, rows: int, width: int, dataLength: int) -> int:
+        out = ctypes.c_int64(0)
+        B200AlgException.ThrowIfFailed(self.L.b200alg_embedding_gradient_temp_bytes(int(rows), int(width), int(dataLength), ctypes.byref(out)))
+        return _ints(out.value)
+
+    def CreateEmbeddingGradient(self, accumulate: bool = False):
+        """Returns ``gradient(stream, tokens, outputGradient, tableGradient, temp, scale=1.0)``: row v of
+        ``tableGradient`` becomes ``scale`` times the sum of the rows of ``outputGradient`` whose token is v,
+        zero where there is none.  With ``accumulate`` the sums are added to what is there.  The sums are held
+        in 32 bits, in the order of the tokens: equal calls give equal bits."""
+        fast, index, add = self._host.embedding_gradient, self._index, int(bool(accumulate))
+
+        def gradient(stream, tokens, outputGradient, tableGradient, temp, scale=1.0):
+            if fast(index, add, stream, tokens, outputGradient, tableGradient, temp, scale):
+                return
+            _check_view(tokens, "tokens")
+            _check_matrix(outputGradient, "outputGradient")
+            _check_matrix(tableGradient, "tableGradient", outputGradient.size(1))
+            _check_index_type(tokens, "tokens")
+            types = _element_code(outputGradient, "outputGradient"), _element_code(tableGradient, "tableGradient")
+            if outputGradient.size(0) < tokens.numel():
+                raise ArgumentOutOfRangeException("outputGradient")
+            _check_temp(temp, self.ComputeEmbeddingGradientTempStorageSize(tableGradient.size(0), tableGradient.size(1), tokens.numel()))
+            self._check_device(tokens, outputGradient, tableGradient, temp)
+            with self.Bind():
+                B200AlgException.ThrowIfFailed(self.L.b200alg_embedding_gradient(
+                    _stream_ptr(stream), _ptr(tokens), tokens.numel(), _stride(tokens), dtype_code(tokens.dtype), _ptr(outputGradient),
+                    _row_stride(outputGradient), types[0], float(scale), _ptr(tableGradient), tableGradient.size(0), tableGradient.size(1),
+                    _row_stride(tableGradient), types[1], add, _ptr(temp), temp.numel() * 4))
+
+        return gradient
+
+    # -- the norm of all gradients, and clipping --
+    def ComputeGradientNormTempStorageSize(self, numViews: int) -> int:
+        out = ctypes.c_int64(0)
+        B200AlgException.ThrowIfFailed(self.L.b200alg_gradient_norm_temp_bytes(int(numViews), ctypes.byref(out)))
+        return _ints(out.value)
+
+    def CreateGradientNorm(self):
+        """Returns ``norm(stream, views, output, temp)``: ``output[0]`` (float32) becomes the square root of the
+        sum of squares over all elements of a list of dense views of any shapes, float32, float16 and
+        bfloat16 side by side."""
+        fast, index = self._host.gradient_norm, self._index
+
+        def norm(stream, views, output, temp):
+            if fast(index, stream, views, output, temp):
+                return
+            _check_views(views, "views")
+            _check_element(output, "output")
+            _check_temp(temp, self.ComputeGradientNormTempStorageSize(len(views)))
+            self._check_device(*views, output, temp)
+            with self.Bind():
+                B200AlgException.ThrowIfFailed(self.L.b200alg_gradient_norm(
+                    _stream_ptr(stream), *self._lists(views), len(views), _ptr(output), _ptr(temp), temp.numel() * 4))
+
+        return norm
+
+    @staticmethod
+    def _lists(views):
+        return (_array(ctypes.c_void_p, [v.data_ptr() for v in views]), _array(ctypes.c_int64, [v.numel() for v in views]),
+                _array(ctypes.c_int, [_ELEMENT_TO_CODE[v.dtype] for v in views]))
+
+    def _clip(self, stream, views, outputs, maxNorm, norm, temp, given):
+        if self._host.gradient_clip(self._index, stream, views, outputs, maxNorm, norm, temp):
+            return
+        _check_views(views, "views")
+        if outputs is not None:
+            _check_views(outputs, "outputs")
+            if [v.numel() for v in outputs] != [v.numel() for v in views]:
+                raise ArgumentOutOfRangeException("outputs")
+        _check_element(norm, "norm")
+        if not float(maxNorm) >= 0.0:
+            raise ArgumentOutOfRangeException("maxNorm")
+        if not given:
+            _check_temp(temp, self.ComputeGradientNormTempStorageSize(len(views)))
+        self._check_device(*views, *(outputs or ()), norm, temp)
+        data, lengths, types = self._lists(views)
+        to = (None, None) if outputs is None else self._lists(outputs)[::2]
+        with self.Bind():
+            if given:
+                B200AlgException.ThrowIfFailed(self.L.b200alg_gradient_scale(
+                    _stream_ptr(stream), data, to[0], lengths, types, to[1], len(views), _ptr(norm), float(maxNorm)))
+            else:
+                B200AlgException.ThrowIfFailed(self.L.b200alg_gradient_clip(
+                    _stream_ptr(stream), data, to[0], lengths, types, to[1], len(views), float(maxNorm), _ptr(norm), _ptr(temp), temp.numel() * 4))
+
+    def CreateGradientClip(self):
+        """Returns ``clip(stream, views, outputs, maxNorm, norm, temp)``: ``norm[0]`` becomes the norm of all
+        views together, and each of ``outputs`` its view times ``min(1, maxNorm / norm)``, rounded to its own
+        type; ``outputs = None`` clips in place.  A norm that is not finite changes no value."""
+        def clip(stream, views, outputs, maxNorm, norm, temp):
+            if temp is None:
+                raise ArgumentNullException("temp")
+            self._clip(stream, views, outputs, maxNorm, norm, temp, False)
+
+        return clip
+
+    def CreateGradientScale(self):
+        """Returns ``scale(stream, views, outputs, maxNorm, norm)``: the second half of ``CreateGradientClip`` by
+        a norm that is in device memory already, combined over ranks for instance."""
+        return lambda stream, views, outputs, maxNorm, norm: self._clip(stream, views, outputs, maxNorm, norm, None, True)
+
+    # -- the balance loss of a router --
+    def ComputeBalanceLossTempStorageSize(self, numExperts: int, dataLength: int) -> int:
+        out = ctypes.c_int64(0)
+        B200AlgException.ThrowIfFailed(self.L.b200alg_balance_loss_temp_bytes(int(numExperts), int(dataLength), ctypes.byref(out)))
+        return _ints(out.value)
+
+    def CreateBalanceLoss(self, coefficient: float):
+        """Returns ``balance(stream, logits, experts, mask, loss, counts, probabilities, temp)`` for logits of
+        tokens x experts and the experts chosen by each token (int32 or int64, tokens x choices): ``loss[0]``
+        (float32) = coefficient * numExperts * sum of count share times mean probability, ``counts`` (int32) how
+        often each expert is chosen and behind them the number of tokens that count, ``probabilities``
+        (float32) the mean softmax.  ``mask`` (bool or uint8, None: all) says which tokens count."""
+        fast, index, factor = self._host.balance_loss, self._index, float(coefficient)
+
+        def balance(stream, logits, experts, mask, loss, counts, probabilities, temp):
+            if fast(index, factor, stream, logits, experts, mask, loss, counts, probabilities, temp):
+                return
+            _check_matrix(logits, "logits")
+            _check_matrix(experts, "experts")
+            _check_index_type(experts, "experts")
+            code = _element_code(logits, "logits")
+            tokens, width = logits.shape
+            if experts.size(0) != tokens:
+                raise ArgumentOutOfRangeException("experts")
+            _check_mask(mask, tokens)
+            _check_element(loss, "loss")
+            _check_element(counts, "counts", torch.int32, width + 1)
+            _check_element(probabilities, "probabilities", torch.float32, width)
+            _check_temp(temp, self.ComputeBalanceLossTempStorageSize(width, tokens))
+            self._check_device(logits, experts, mask, loss, counts, probabilities, temp)
+            with self.Bind():
+                B200AlgException.ThrowIfFailed(self.L.b200alg_balance_loss(
+                    _stream_ptr(stream), _ptr(logits), tokens, width, _row_stride(logits), code, _ptr(experts), experts.size(1), _row_stride(experts),
+                    dtype_code(experts.dtype), _ptr(mask), factor, _ptr(loss), _ptr(counts), _ptr(probabilities), _ptr(temp), temp.numel() * 4))
+
+        return balance
+
+    def CreateBalanceLossGradient(self, coefficient: float, choices: int, accumulate: bool = False):
+        """Returns ``gradient(stream, logits, mask, counts, lossGradient, logitsGradient)``: the gradient of the
+        balance loss in its logits times ``lossGradient[0]`` (float32), with the counts as the loss gave them (or
+        their sums over ranks) taken as constants; zero for tokens that do not count.  With ``accumulate`` it is
+        added to what is there."""
+        fast, index, factor, add = self._host.balance_loss_gradient, self._index, float(coefficient), int(bool(accumulate))
+
+        def gradient(stream, logits, mask, counts, lossGradient, logitsGradient):
+            if fast(index, factor, choices, add, stream, logits, mask, counts, lossGradient, logitsGradient):
+                return
+            _check_matrix(logits, "logits")
+            code = _element_code(logits, "logits")
+            tokens, width = logits.shape
+            _check_mask(mask, tokens)
+            _check_element(counts, "counts", torch.int32, width + 1)
+            _check_element(lossGradient, "lossGradient")
+            _check_matrix(logitsGradient, "logitsGradient", width)
+            if logitsGradient.size(0) != tokens:
+                raise ArgumentOutOfRangeException("logitsGradient")
+            if logitsGradient.dtype != logits.dtype:
+                raise InvalidOperationException(f"logitsGradient: element type {logitsGradient.dtype}, expected {logits.dtype}")
+            self._check_device(logits, mask, counts, lossGradient, logitsGradient)
+            with self.Bind():
+                B200AlgException.ThrowIfFailed(self.L.b200alg_balance_loss_gradient(
+                    _stream_ptr(stream), _ptr(logits), tokens, width, _row_stride(logits), code, _ptr(mask), _ptr(counts), int(choices), factor,
+                    _ptr(lossGradient), _ptr(logitsGradient), _row_stride(logitsGradient), add))
+
+        return gradient
 
     def CheckDeviceStatus(self, stream, temp: torch.Tensor) -> None:
         """Synchronises and raises if a bounded device-side wait ran out during a call that

@@ -17,6 +17,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <vector>
 
 #include "../../include/b200alg.h"
 
@@ -36,7 +37,17 @@ namespace {
     X(histogram) \
     X(initialize) \
     X(unique_temp_bytes) \
-    X(unique_to_host)
+    X(unique_to_host) \
+    X(embedding) \
+    X(embedding_gradient_temp_bytes) \
+    X(embedding_gradient) \
+    X(gradient_norm_temp_bytes) \
+    X(gradient_norm) \
+    X(gradient_scale) \
+    X(gradient_clip) \
+    X(balance_loss_temp_bytes) \
+    X(balance_loss) \
+    X(balance_loss_gradient)
 struct Library {
 #define B200ALG_MEMBER(name) decltype(&b200alg_##name) name;
     B200ALG_ENTRY_POINTS(B200ALG_MEMBER)
@@ -353,6 +364,216 @@ PyObject *initialize(PyObject *, PyObject *const *a, Py_ssize_t count) {
     });
 }
 
+// ---- operators of a training step ---------------------------------------------------------------
+
+// Their element types; -1 for any other.
+int element_code_of(at::ScalarType t) {
+    switch (t) {
+    case at::kHalf: return B200ALG_F16;
+    case at::kBFloat16: return B200ALG_BF16;
+    case at::kFloat: return B200ALG_F32;
+    default: return -1;
+    }
+}
+
+struct Matrix {
+    void *data = nullptr;
+    int64_t rows = 0, width = 0, stride = 0;
+    int code = -1;
+};
+
+// A two-dimensional CUDA view on `device` whose rows are dense; `indices`: of int32 or int64, else of one of the
+// operators' element types.
+bool matrix_of(PyObject *o, int device, bool indices, Matrix &m) {
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (t.dim() != 2 || !t.is_cuda() || t.get_device() != device) return false;
+    m.code = indices ? code_of(t.scalar_type()) : element_code_of(t.scalar_type());
+    if (indices ? m.code != B200ALG_I32 && m.code != B200ALG_I64 : m.code < 0) return false;
+    m.rows = t.size(0), m.width = t.size(1);
+    if (m.width > 1 && t.stride(1) != 1) return false;
+    m.stride = m.rows > 1 ? t.stride(0) : m.width;
+    m.data = t.data_ptr();
+    return true;
+}
+
+bool indices_of(PyObject *o, int device, View &v) {
+    return view_of(o, device, -1, v) && (v.code == B200ALG_I32 || v.code == B200ALG_I64);
+}
+
+// A view of at least one float.
+bool float_of(PyObject *o, int device, View &v) { return view_of(o, device, B200ALG_F32, v) && v.n >= 1; }
+
+// embedding(device, stream, table, tokens, output, scale)
+PyObject *embedding(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded([&] {
+        const int device = count == 6 ? device_of(a[0]) : -1;
+        Matrix table, out;
+        View tokens;
+        void *stream;
+        if (device < 0 || !matrix_of(a[2], device, false, table) || !indices_of(a[3], device, tokens) || !matrix_of(a[4], device, false, out)) return false;
+        if (out.width != table.width || out.rows < tokens.n || !stream_of(a[1], device, stream)) return false;
+        const double scale = PyFloat_AsDouble(a[5]);
+        if (PyErr_Occurred()) return false;
+        return released([&] {
+                   return lib.embedding(stream, table.data, table.rows, table.width, table.stride, table.code, tokens.data, tokens.n, tokens.stride,
+                                        tokens.code, scale, out.data, out.stride, out.code);
+               }) == B200ALG_OK;
+    });
+}
+
+// embedding_gradient(device, accumulate, stream, tokens, upstream, gradient, temp, scale)
+PyObject *embedding_gradient(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded([&] {
+        const int device = count == 8 ? device_of(a[0]) : -1;
+        const int accumulate = int_of(a[1]);
+        Matrix upstream, gradient;
+        View tokens, temp;
+        void *stream;
+        int64_t need = 0;
+        if (device < 0 || !indices_of(a[3], device, tokens) || !matrix_of(a[4], device, false, upstream) || !matrix_of(a[5], device, false, gradient))
+            return false;
+        if (upstream.width != gradient.width || upstream.rows < tokens.n || !stream_of(a[2], device, stream)) return false;
+        const double scale = PyFloat_AsDouble(a[7]);
+        if (PyErr_Occurred()) return false;
+        if (lib.embedding_gradient_temp_bytes(gradient.rows, gradient.width, tokens.n, &need) != B200ALG_OK || !temp_of(a[6], device, need, temp))
+            return false;
+        return released([&] {
+                   return lib.embedding_gradient(stream, tokens.data, tokens.n, tokens.stride, tokens.code, upstream.data, upstream.stride,
+                                                 upstream.code, scale, gradient.data, gradient.rows, gradient.width, gradient.stride, gradient.code,
+                                                 accumulate, temp.data, temp.n * 4);
+               }) == B200ALG_OK;
+    });
+}
+
+// The dense views of a list or tuple, of any shape.
+struct ViewList {
+    std::vector<void *> data;
+    std::vector<int64_t> lengths;
+    std::vector<int> codes;
+    bool from(PyObject *o, int device) {
+        if (!PyList_Check(o) && !PyTuple_Check(o)) return false;
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+        PyObject **item = PySequence_Fast_ITEMS(o);
+        data.resize(n), lengths.resize(n), codes.resize(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            if (!THPVariable_Check(item[i])) return false;
+            const at::Tensor &t = THPVariable_Unpack(item[i]);
+            if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous()) return false;
+            codes[i] = element_code_of(t.scalar_type());
+            if (codes[i] < 0) return false;
+            lengths[i] = t.numel();
+            data[i] = t.data_ptr();
+        }
+        return true;
+    }
+};
+
+// gradient_norm(device, stream, views, norm, temp)
+PyObject *gradient_norm(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded([&] {
+        const int device = count == 5 ? device_of(a[0]) : -1;
+        ViewList views;
+        View norm, temp;
+        void *stream;
+        int64_t need = 0;
+        if (device < 0 || !views.from(a[2], device) || !float_of(a[3], device, norm) || !stream_of(a[1], device, stream)) return false;
+        const int64_t n = (int64_t)views.data.size();
+        if (lib.gradient_norm_temp_bytes(n, &need) != B200ALG_OK || !temp_of(a[4], device, need, temp)) return false;
+        return released([&] {
+                   return lib.gradient_norm(stream, views.data.data(), views.lengths.data(), views.codes.data(), n, (float *)norm.data, temp.data,
+                                            temp.n * 4);
+               }) == B200ALG_OK;
+    });
+}
+
+// gradient_clip(device, stream, views, outputs or None, max_norm, norm, temp or None): with temp the norm is taken,
+// without it it is given
+PyObject *gradient_clip(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded([&] {
+        const int device = count == 7 ? device_of(a[0]) : -1;
+        ViewList views, outputs;
+        View norm, temp;
+        void *stream;
+        int64_t need = 0;
+        const bool apart = a[3] != Py_None;
+        if (device < 0 || !views.from(a[2], device) || (apart && !outputs.from(a[3], device)) || !float_of(a[5], device, norm)) return false;
+        if ((apart && outputs.lengths != views.lengths) || !stream_of(a[1], device, stream)) return false;
+        const double max_norm = PyFloat_AsDouble(a[4]);
+        if (PyErr_Occurred()) return false;
+        const int64_t n = (int64_t)views.data.size();
+        void *const *to = apart ? outputs.data.data() : nullptr;
+        const int *types = apart ? outputs.codes.data() : nullptr;
+        if (a[6] == Py_None)
+            return released([&] {
+                       return lib.gradient_scale(stream, views.data.data(), to, views.lengths.data(), views.codes.data(), types, n,
+                                                 (const float *)norm.data, max_norm);
+                   }) == B200ALG_OK;
+        if (lib.gradient_norm_temp_bytes(n, &need) != B200ALG_OK || !temp_of(a[6], device, need, temp)) return false;
+        return released([&] {
+                   return lib.gradient_clip(stream, views.data.data(), to, views.lengths.data(), views.codes.data(), types, n, max_norm,
+                                            (float *)norm.data, temp.data, temp.n * 4);
+               }) == B200ALG_OK;
+    });
+}
+
+// A mask of bytes or truth values for at least `tokens` tokens, or None.
+bool mask_of(PyObject *o, int device, int64_t tokens, void *&p) {
+    p = nullptr;
+    if (o == Py_None) return true;
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (t.dim() != 1 || !t.is_cuda() || t.get_device() != device || t.numel() < tokens) return false;
+    if ((t.scalar_type() != at::kBool && t.scalar_type() != at::kByte) || (t.numel() > 1 && t.stride(0) != 1)) return false;
+    p = t.data_ptr();
+    return true;
+}
+
+// balance_loss(device, coefficient, stream, logits, experts, mask or None, loss, counts, probabilities, temp)
+PyObject *balance_loss(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded([&] {
+        const int device = count == 10 ? device_of(a[0]) : -1;
+        const double coefficient = PyFloat_AsDouble(a[1]);
+        Matrix logits, chosen;
+        View loss, counts, probabilities, temp;
+        void *stream, *mask;
+        int64_t need = 0;
+        if (device < 0 || !matrix_of(a[3], device, false, logits) || !matrix_of(a[4], device, true, chosen)) return false;
+        if (chosen.rows != logits.rows || !mask_of(a[5], device, logits.rows, mask) || !float_of(a[6], device, loss)) return false;
+        if (!view_of(a[7], device, B200ALG_I32, counts) || counts.stride != 1 || counts.n < logits.width + 1) return false;
+        if (!view_of(a[8], device, B200ALG_F32, probabilities) || probabilities.stride != 1 || probabilities.n < logits.width) return false;
+        if (lib.balance_loss_temp_bytes(logits.width, logits.rows, &need) != B200ALG_OK || !temp_of(a[9], device, need, temp)) return false;
+        if (!stream_of(a[2], device, stream) || PyErr_Occurred()) return false;
+        return released([&] {
+                   return lib.balance_loss(stream, logits.data, logits.rows, logits.width, logits.stride, logits.code, chosen.data, chosen.width,
+                                           chosen.stride, chosen.code, mask, coefficient, (float *)loss.data, (int32_t *)counts.data,
+                                           (float *)probabilities.data, temp.data, temp.n * 4);
+               }) == B200ALG_OK;
+    });
+}
+
+// balance_loss_gradient(device, coefficient, choices, accumulate, stream, logits, mask or None, counts, loss_gradient, gradient)
+PyObject *balance_loss_gradient(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded([&] {
+        const int device = count == 10 ? device_of(a[0]) : -1;
+        const double coefficient = PyFloat_AsDouble(a[1]);
+        const int choices = int_of(a[2]), accumulate = int_of(a[3]);
+        Matrix logits, gradient;
+        View counts, loss_gradient;
+        void *stream, *mask;
+        if (device < 0 || !matrix_of(a[5], device, false, logits) || !mask_of(a[6], device, logits.rows, mask)) return false;
+        if (!view_of(a[7], device, B200ALG_I32, counts) || counts.stride != 1 || counts.n < logits.width + 1) return false;
+        if (!float_of(a[8], device, loss_gradient) || !matrix_of(a[9], device, false, gradient)) return false;
+        if (gradient.rows != logits.rows || gradient.width != logits.width || gradient.code != logits.code) return false;
+        if (!stream_of(a[4], device, stream) || PyErr_Occurred()) return false;
+        return released([&] {
+                   return lib.balance_loss_gradient(stream, logits.data, logits.rows, logits.width, logits.stride, logits.code, mask,
+                                                    (const int32_t *)counts.data, choices, coefficient, (const float *)loss_gradient.data,
+                                                    gradient.data, gradient.stride, accumulate);
+               }) == B200ALG_OK;
+    });
+}
+
 // bind(addresses): one address per name in ENTRY_POINTS
 PyObject *bind(PyObject *, PyObject *addresses) {
     constexpr Py_ssize_t kCount = sizeof(Library) / sizeof(void *);
@@ -369,7 +590,8 @@ PyObject *bind(PyObject *, PyObject *addresses) {
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr}, FAST(sort_keys), FAST(sort_pairs), FAST(scan), FAST(reduce), FAST(reduce_value),
-                         FAST(histogram), FAST(unique), FAST(initialize), {nullptr, nullptr, 0, nullptr}};
+                         FAST(histogram), FAST(unique), FAST(initialize), FAST(embedding), FAST(embedding_gradient),
+                         FAST(gradient_norm), FAST(gradient_clip), FAST(balance_loss), FAST(balance_loss_gradient), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of the algorithm calls.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

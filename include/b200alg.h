@@ -31,7 +31,8 @@ extern "C" {
 typedef enum {
     B200ALG_I8 = 0, B200ALG_U8 = 1, B200ALG_I16 = 2, B200ALG_U16 = 3,
     B200ALG_I32 = 4, B200ALG_U32 = 5, B200ALG_I64 = 6, B200ALG_U64 = 7,
-    B200ALG_F16 = 8, B200ALG_F32 = 9, B200ALG_F64 = 10
+    B200ALG_F16 = 8, B200ALG_F32 = 9, B200ALG_F64 = 10,
+    B200ALG_BF16 = 11 /* the operators of a training step only */
 } b200alg_dtype;
 
 /* Scan / reduce operations: Add*, Max*, Min* of ScanReduceOperations.tt:20-26. */
@@ -236,6 +237,80 @@ int b200alg_unique_to_host(void *stream, void *data, int64_t n, int dtype, int64
 int b200alg_run_length_encode_temp_bytes(int dtype, int64_t n, int64_t *out_bytes);
 int b200alg_run_length_encode(void *stream, const void *data, int64_t n, int dtype, void *values, int64_t *lengths,
                               int64_t *num_runs, void *temp, int64_t temp_bytes);
+
+/* ---- operators of a language model's training step ----------------------------------
+ * Built from the primitives above: embedding gradients from sorted pairs, the norm of all
+ * gradients from a reduction over a list of views, the balance loss of a router from a
+ * histogram.  No counterpart in the reference.
+ *
+ * Element types are F32, F16 and BF16; sums are held in 32 bits or more, in an order that
+ * depends on sizes only, and results are rounded once.  Token and expert indices are I32 or
+ * I64.  Matrices are row-major with rows `*_stride` elements apart; what lies between the
+ * width of a row and the next row is neither read nor written.  Outputs overlap no input
+ * (b200alg_gradient_clip and b200alg_gradient_scale may work in place).  At most 2^31 - 1
+ * rows, columns and tokens (B200ALG_TOO_LARGE). */
+
+/* out[i, 0..width) = scale * table[tokens[i], 0..width) for i in [0, n); zeros where
+ * tokens[i] lies outside [0, rows). */
+int b200alg_embedding(void *stream, const void *table, int64_t rows, int64_t width, int64_t row_stride, int dtype,
+                      const void *tokens, int64_t n, int64_t token_stride, int token_dtype, double scale, void *out,
+                      int64_t out_stride, int out_dtype);
+
+/* The gradient of the lookup in its table: gradient[v, :] = scale * the sum of upstream[i, :]
+ * over all i with tokens[i] == v, in the order of i; every row of the table's gradient is
+ * written, rows that no token names with zeros.  With accumulate != 0 the sums are added to
+ * what `gradient` holds, and rows that no token names are left alone.  Tokens outside
+ * [0, rows) add to nothing.  b200alg_device_status(temp) holds for this call. */
+int b200alg_embedding_gradient_temp_bytes(int64_t rows, int64_t width, int64_t n, int64_t *out_bytes);
+int b200alg_embedding_gradient(void *stream, const void *tokens, int64_t n, int64_t token_stride, int token_dtype,
+                               const void *upstream, int64_t upstream_stride, int upstream_dtype, double scale,
+                               void *gradient, int64_t rows, int64_t width, int64_t row_stride, int dtype,
+                               int accumulate, void *temp, int64_t temp_bytes);
+
+/* norm[0] (float, device) = sqrt(sum of x^2) over all elements of `count` dense views.  The
+ * lists (views, lengths, dtypes) are host memory and are not looked at after return; a view
+ * may be empty, and no view at all has norm 0.  Squares that 32 bits do not hold are taken in
+ * 64: the norm is right wherever it is a float itself.  At most 2^38 elements in all. */
+int b200alg_gradient_norm_temp_bytes(int64_t count, int64_t *out_bytes);
+int b200alg_gradient_norm(void *stream, const void *const *views, const int64_t *lengths, const int *dtypes,
+                          int64_t count, float *norm, void *temp, int64_t temp_bytes);
+
+/* outputs[v][i] = views[v][i] * min(1, max_norm / norm[0]) in outputs' own types; with
+ * outputs == NULL (and out_dtypes NULL) in place.  A norm that is not finite changes nothing:
+ * the values pass as they are.  max_norm >= 0.  out_dtypes == NULL: the views' types.
+ * norm is read on the device: between b200alg_gradient_norm and this call it may be combined
+ * with other ranks' norms. */
+int b200alg_gradient_scale(void *stream, const void *const *views, void *const *outputs, const int64_t *lengths,
+                           const int *dtypes, const int *out_dtypes, int64_t count, const float *norm,
+                           double max_norm);
+
+/* Both: norm[0] = the norm of the views, then clipped by it. */
+int b200alg_gradient_clip(void *stream, const void *const *views, void *const *outputs, const int64_t *lengths,
+                          const int *dtypes, const int *out_dtypes, int64_t count, double max_norm, float *norm,
+                          void *temp, int64_t temp_bytes);
+
+/* The balance loss of a router that sends each of `tokens` tokens to `choices` of `experts`
+ * experts (at most 1024 of each): with p_t = softmax(logits[t, :]), c_e = how often expert e
+ * is chosen (chosen[t, j]; values outside [0, experts) are no choice) and P_e = the mean of
+ * p_te, loss[0] = coefficient * experts * sum over e of c_e / (T' choices) * P_e.  Only
+ * tokens with mask[t] != 0 (bytes; NULL: all) count, T' of them; the others' logits and
+ * choices are not read.  A row of nothing but -inf has p = 0.  counts[0..experts) = c_e,
+ * counts[experts] = T' (int32), probabilities[e] = P_e (float); T' = 0 gives zeros. */
+int b200alg_balance_loss_temp_bytes(int64_t experts, int64_t tokens, int64_t *out_bytes);
+int b200alg_balance_loss(void *stream, const void *logits, int64_t tokens, int64_t experts, int64_t logits_stride,
+                         int dtype, const void *chosen, int64_t choices, int64_t chosen_stride, int chosen_dtype,
+                         const void *mask, double coefficient, float *loss, int32_t *counts, float *probabilities,
+                         void *temp, int64_t temp_bytes);
+
+/* Its gradient in the logits, the counts taken as constants (`counts` as the call above gives
+ * them, or their sums over ranks): gradient[t, e] = loss_gradient[0] * coefficient * experts /
+ * (T'^2 choices) * p_te * (c_e - sum over j of c_j p_tj), zero for tokens that the mask leaves
+ * out.  With accumulate != 0 it is added to what `gradient` holds.  gradient has the logits'
+ * type. */
+int b200alg_balance_loss_gradient(void *stream, const void *logits, int64_t tokens, int64_t experts,
+                                  int64_t logits_stride, int dtype, const void *mask, const int32_t *counts,
+                                  int64_t choices, double coefficient, const float *loss_gradient, void *gradient,
+                                  int64_t gradient_stride, int accumulate);
 
 /* Device-side waits (decoupled look-back) are bounded; when one runs out the kernel
  * records it in `temp` and finishes.  This call copies that record back and
