@@ -11,25 +11,33 @@
 #include <math.h>
 #include <type_traits>
 
+#include <cooperative_groups.h>
+
 #include "elements.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace b200alg {
 
-constexpr int kBalanceThreads = 256;
+constexpr int kBalanceThreads = 512;  // (256, and so twice the shares to add up: 28.7 us instead of 25.2 for 262144 tokens and 128 experts in bf16)
 constexpr int kBalanceWarps = kBalanceThreads / 32;
 constexpr int kMostExperts = 1024;
-constexpr int kBalanceBlocksPerSm = 4;
-constexpr int kMostBalanceBlocks = 148 * kBalanceBlocksPerSm;
+constexpr int kBalanceCluster = 8;  // blocks that add up in each other's shared memory
+constexpr int kMostBalanceBlocks = 148 * 3;
+constexpr int kFinishThreads = 1024;
+constexpr int kIndexSlots = 2;        // indices of a row that a lane fetches ahead
+constexpr int kShareAhead = 8;      // blocks' shares that a thread has in flight
 
 struct BalanceCall {
     int64_t tokens, logits_stride;
     int experts, choices;
     const unsigned char *mask;  // of the tokens that count, NULL: all do
-    int lanes;                  // of a row: a power of two
     int groups;                 // of a row
 };
 
 __host__ __device__ constexpr int padded_bins(int experts) { return (experts + 4) / 4 * 4; }
+constexpr int kGradientWarps = 8;
+constexpr size_t kBalanceSmem = (size_t)padded_bins(kMostExperts) * (2 + kBalanceWarps) * 4;  // of balance_kernel at most
 
 __device__ __forceinline__ float exp2_approximate(float x) {  // 2^x; below 2^-126 zero
     float y;
@@ -37,251 +45,479 @@ __device__ __forceinline__ float exp2_approximate(float x) {  // 2^x; below 2^-1
     return y;
 }
 
-// A row's logits in the registers of `lanes` lanes: group c of lane l holds the columns (c * lanes + l) * V on.
-template <typename T, int V, int C> struct RouterRow {
-    Group<T, V> raw[C];
+template <typename T> struct LowestBits;  // -inf, in each part of a word
+template <> struct LowestBits<float> { static constexpr unsigned int value = 0xFF800000u; };
+template <> struct LowestBits<__half> { static constexpr unsigned int value = 0xFC00FC00u; };
+template <> struct LowestBits<__nv_bfloat16> { static constexpr unsigned int value = 0xFF80FF80u; };
 
-    __device__ __forceinline__ void load(const T *p, const BalanceCall &call, int lane_of_row) {
+// How a row lies in a warp: LANES lanes share it, each with C groups of V elements; group c of lane l holds the columns
+// (c * LANES + l) * V on.  A lane has U rows in flight.
+template <int V_, int C_, int LANES_, int U_> struct RowShape {
+    static constexpr int V = V_, C = C_, LANES = LANES_, U = U_, E = V_ * C_;
+    static constexpr int ROWS = 32 / LANES_;  // of a warp at a time
+};
+
+// Two floats in one instruction, which is what these kernels are made of.
+struct Pair {
+    unsigned long long bits;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void apart(float &a, float &b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return r;
+}
+
+template <typename T, typename S> struct RouterRow {
+    Group<T, S::V> raw[S::C];
+
+    // -inf in the places that the row does not have, and in all of a row that does not count: their exp is zero.
+    __device__ __forceinline__ void load(const T *p, bool there, int groups, int lane_of_row) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int g = c * call.lanes + lane_of_row;
-            if (g < call.groups) raw[c].load(p + (int64_t)g * V);
+        for (int c = 0; c < S::C; ++c) {
+#pragma unroll
+            for (int i = 0; i < Group<T, S::V>::kWords; ++i) raw[c].w[i] = LowestBits<T>::value;
+            const int g = c * S::LANES + lane_of_row;
+            if (there && g < groups) raw[c].load(p + g * S::V);
         }
     }
-    // e = exp(x - max x), zero in places that the row does not have; all lanes take part.
-    __device__ __forceinline__ void exponentials(float (&e)[C * V], const BalanceCall &call, int lane_of_row, bool there) const {
+    // The largest value of the row (a NaN is left out here and comes back from the exponentials); all lanes take part.
+    __device__ __forceinline__ float top() const {
         float top = -INFINITY;
+        if constexpr (sizeof(T) == 2 && S::V > 1) {  // two at a time
+            using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            unsigned int most = LowestBits<T>::value;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const bool in = there && c * call.lanes + lane_of_row < call.groups;
+            for (int c = 0; c < S::C; ++c)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                e[c * V + v] = in ? raw[c].get(v) : -INFINITY;
-                top = fmaxf(top, e[c * V + v]);  // (a NaN is left out here and comes back below)
-            }
+                for (int i = 0; i < Group<T, S::V>::kWords; ++i) {
+                    const T2 m = __hmax2(*reinterpret_cast<const T2 *>(&most), *reinterpret_cast<const T2 *>(&raw[c].w[i]));
+                    most = *reinterpret_cast<const unsigned int *>(&m);
+                }
+            Group<T, 2> two;
+            two.w[0] = most;
+            top = fmaxf(two.get(0), two.get(1));
+        } else {
+#pragma unroll
+            for (int c = 0; c < S::C; ++c)
+#pragma unroll
+                for (int v = 0; v < S::V; ++v) top = fmaxf(top, raw[c].get(v));
         }
-        for (int d = call.lanes >> 1; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (top == -INFINITY) top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < C * V; ++i) e[i] = exp2_approximate((e[i] - top) * 1.4426950408889634f);
+        for (int d = S::LANES >> 1; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        return top;
+    }
+    __device__ __forceinline__ float element(int i) const { return raw[i / S::V].get(i % S::V); }
+    // e = exp(x - max x) times a power of two below 2 that is the row's own and leaves with its sum.  x log2(e) less a
+    // whole number is one fused operation, rounded once; where the largest value is so large that its product with
+    // log2(e) is not near a whole number any more, x - max x is taken first.
+    __device__ __forceinline__ void exponentials(Pair (&e)[S::E / 2]) const {
+        constexpr float kLog2e = 1.4426950408889634f;
+        float most = top();
+        if (most == -INFINITY) most = 0.0f;
+        if (fabsf(most) <= 0x1p20f) {
+            const float whole = -rintf(most * kLog2e);
+            const Pair by(kLog2e, kLog2e), from(whole, whole);
+#pragma unroll
+            for (int i = 0; i < S::E / 2; ++i) {
+                float a, b;
+                fma(Pair(element(2 * i), element(2 * i + 1)), by, from).apart(a, b);
+                e[i] = Pair(exp2_approximate(a), exp2_approximate(b));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::E / 2; ++i)
+                e[i] = Pair(exp2_approximate((element(2 * i) - most) * kLog2e), exp2_approximate((element(2 * i + 1) - most) * kLog2e));
+        }
     }
 };
 
-__device__ __forceinline__ float row_sum(float x, int lanes) {
-    for (int d = lanes >> 1; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+template <int LANES> __device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+    for (int d = LANES >> 1; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
     return x;
 }
+__device__ __forceinline__ float sum_of(Pair x) {
+    float a, b;
+    x.apart(a, b);
+    return a + b;
+}
 
-// What a block found, in temp: sums of p by expert, counts by expert, tokens that count.
+// 1 / x of a row's sum: between 1/2 and twice the number of experts, zero where every logit is -inf, NaN where one is.
+__device__ __forceinline__ float inverse_of(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return x == 0.0f ? 0.0f : y;
+}
+
+// What the blocks found, in temp: sums of p by expert, and counts by expert with the tokens that count behind them.
 struct BalanceShares {
-    float *sums;      // [blocks][experts]
+    float *sums;           // [blocks][experts]
     unsigned int *counts;  // [blocks][experts + 1]
 };
 
-// The shares of all blocks as the call's results, by one block.
-__device__ void finish_balance(const BalanceShares &shares, int blocks, int experts, int choices, double coefficient, float *loss, int *counts,
-                               float *probabilities) {
-    __shared__ unsigned int valid;
-    __shared__ double part[kBalanceWarps];
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        unsigned int n = 0u;
-        for (int b = threadIdx.x; b < blocks; b += 32) n += __ldcg(shares.counts + (int64_t)b * (experts + 1) + experts);
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (threadIdx.x == 0) valid = n;
-    }
-    __syncthreads();
+struct BalanceResult {
+    double factor;  // coefficient * experts / choices
+    float *loss;
+    int *counts;
+    float *probabilities;
+};
+
+__device__ __forceinline__ double sum_of_warp(double sum) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum;
+}
+
+// The results from the sums and counts of all tokens, by the blocks of a cluster that are known to run: `sums` and
+// `counts` hold this block's columns [first, last) of the experts; `valid` tokens count.
+template <int THREADS>
+__device__ void finish_balance(const float *sums, const unsigned int *counts, int first, int last, unsigned int valid, int experts,
+                               const BalanceResult &to) {
+    __shared__ double share[kBalanceCluster], part[THREADS / 32];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31;
     const double inverse = valid ? 1.0 / valid : 0.0;
     double sum = 0.0;
-    for (int e = threadIdx.x; e < experts; e += kBalanceThreads) {
-        double p = 0.0;
-        unsigned int n = 0u;
-        for (int b = 0; b < blocks; ++b) {
-            p += __ldcg(shares.sums + (int64_t)b * experts + e);
-            n += __ldcg(shares.counts + (int64_t)b * (experts + 1) + e);
-        }
-        p *= inverse;
-        counts[e] = (int)n;
-        probabilities[e] = (float)p;
-        sum += n * inverse / choices * p;
+    for (int e = first + threadIdx.x; e < last; e += THREADS) {
+        const double p = sums[e - first] * inverse;
+        to.counts[e] = (int)counts[e - first];
+        to.probabilities[e] = (float)p;
+        sum += counts[e - first] * p;
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, d);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+    sum = sum_of_warp(sum);
+    if (lane == 0) part[threadIdx.x >> 5] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kBalanceWarps; ++w) sum += part[w];
-        *loss = (float)(coefficient * experts * sum);
-        counts[experts] = (int)valid;
+    if (threadIdx.x < 32) {
+        sum = sum_of_warp(lane < THREADS / 32 ? part[lane] : 0.0);
+        if (lane == 0) *cluster.map_shared_rank(share + rank, 0) = sum;
+    }
+    cluster.sync();
+    if (rank == 0 && threadIdx.x < 32) {
+        sum = sum_of_warp(lane < blocks ? share[lane] : 0.0);
+        if (lane == 0) {
+            *to.loss = (float)(sum * inverse * to.factor);
+            to.counts[experts] = (int)valid;
+        }
     }
 }
 
-template <typename T, int V, int C>
-__global__ void __launch_bounds__(kBalanceThreads)
-balance_kernel(BalanceCall call, const T *__restrict__ logits, IndexView chosen, FastDivide by_choices, BalanceShares shares, double coefficient,
-               float *loss, int *counts, float *probabilities) {
+template <typename T, typename S>
+__global__ void __launch_bounds__(kBalanceThreads, S::E <= 16 ? 2 : 1)
+balance_kernel(BalanceCall call, const T *__restrict__ logits, IndexView chosen, BalanceShares shares, BalanceResult to, int alone) {
     grid_dependency_release();
-    extern __shared__ unsigned char smem[];
-    unsigned int *bins = reinterpret_cast<unsigned int *>(smem);                  // [experts + 1]
-    float *sums = reinterpret_cast<float *>(bins + padded_bins(call.experts));  // [warps][experts]
-    for (int e = threadIdx.x; e <= call.experts; e += kBalanceThreads) bins[e] = 0u;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int experts = call.experts;
+    unsigned int *bins = reinterpret_cast<unsigned int *>(smem);                 // [experts + 1]
+    float *sums = reinterpret_cast<float *>(bins + padded_bins(experts));        // [warps][experts], then [experts]
+    for (int e = threadIdx.x; e <= experts; e += kBalanceThreads) bins[e] = 0u;
     __syncthreads();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t begin = call.tokens * blockIdx.x / gridDim.x, end = call.tokens * (blockIdx.x + 1) / gridDim.x;
+    const int lane_of_row = lane & (S::LANES - 1), row_of_warp = lane / S::LANES;
+    const unsigned int tokens = (unsigned int)call.tokens;
+    const unsigned int apart = gridDim.x * (kBalanceWarps * S::ROWS);  // rows that the grid takes at a time
 
-    // counts
+    // An index that no expert has is out of range in 32 bits, too.
+    auto index_at = [&](int64_t at) -> unsigned int {
+        if (!chosen.wide) return reinterpret_cast<const unsigned int *>(chosen.p)[at];
+        const uint2 w = reinterpret_cast<const uint2 *>(chosen.p)[at];
+        return w.y ? ~0u : w.x;
+    };
     unsigned int valid = 0u;
-    for (int64_t t = begin + threadIdx.x; t < end; t += kBalanceThreads) valid += call.mask ? call.mask[t] != 0 : 1u;
+    Pair sum[S::E / 2];
+#pragma unroll
+    for (int i = 0; i < S::E / 2; ++i) sum[i] = Pair(0.0f, 0.0f);
+    // (no row's number passes 32 bits: tokens is at most 2^31 - 1, the grid takes fewer than 2^20 rows at a time)
+    // A lane's rows come round in turn: each is loaded again, for the row U steps on, as soon as its values are in use, and
+    // whether that row counts is known a round before.
+    RouterRow<T, S> r[S::U];
+    bool there[S::U], soon[S::U];
+    unsigned int index[S::U][kIndexSlots];
+    auto counts_in = [&](unsigned int row) { return row < tokens && (!call.mask || call.mask[row]); };
+    auto fetch = [&](int u, unsigned int row) {
+        r[u].load(logits + row * call.logits_stride, there[u], call.groups, lane_of_row);
+#pragma unroll
+        for (int k = 0; k < kIndexSlots; ++k) {
+            const int j = lane_of_row + k * S::LANES;
+            index[u][k] = there[u] && j < call.choices ? index_at(row * chosen.stride + j) : ~0u;
+        }
+    };
+    unsigned int t = (blockIdx.x * kBalanceWarps + warp) * S::ROWS + row_of_warp;
+#pragma unroll
+    for (int u = 0; u < S::U; ++u) there[u] = counts_in(t + u * apart);
+#pragma unroll
+    for (int u = 0; u < S::U; ++u) {
+        fetch(u, t + u * apart);
+        soon[u] = counts_in(t + (u + S::U) * apart);
+    }
+    for (; t - row_of_warp < tokens; t += apart * S::U) {
+#pragma unroll
+        for (int u = 0; u < S::U; ++u) {
+            const unsigned int row = t + u * apart;
+            if (row - row_of_warp >= tokens) break;
+            valid += there[u] && lane_of_row == 0;
+#pragma unroll
+            for (int k = 0; k < kIndexSlots; ++k)
+                if (index[u][k] < (unsigned int)experts) atomicAdd(bins + index[u][k], 1u);
+            if (there[u])
+                for (int j = lane_of_row + kIndexSlots * S::LANES; j < call.choices; j += S::LANES) {
+                    const unsigned int e = index_at(row * chosen.stride + j);
+                    if (e < (unsigned int)experts) atomicAdd(bins + e, 1u);
+                }
+            Pair e[S::E / 2];
+            r[u].exponentials(e);
+            there[u] = soon[u];
+            fetch(u, row + apart * S::U);
+            soon[u] = counts_in(row + apart * (2 * S::U));
+            Pair whole = e[0];
+#pragma unroll
+            for (int i = 1; i < S::E / 2; ++i) whole = whole + e[i];
+            const float inverse = inverse_of(row_sum<S::LANES>(sum_of(whole)));
+            const Pair by(inverse, inverse);
+#pragma unroll
+            for (int i = 0; i < S::E / 2; ++i) sum[i] = fma(e[i], by, sum[i]);
+        }
+    }
     valid = __reduce_add_sync(0xffffffffu, valid);
-    if (lane == 0) atomicAdd(bins + call.experts, valid);
-    const unsigned int ids = (unsigned int)((end - begin) * call.choices);
-    for (unsigned int i = threadIdx.x; i < ids; i += kBalanceThreads) {
-        const unsigned int t = by_choices(i), j = i - t * call.choices;
-        if (call.mask && !call.mask[begin + t]) continue;
-        const int64_t e = chosen.wide ? reinterpret_cast<const long long *>(chosen.p)[(begin + t) * chosen.stride + j]
-                                      : reinterpret_cast<const int *>(chosen.p)[(begin + t) * chosen.stride + j];
-        if (e >= 0 && e < call.experts) atomicAdd(bins + e, 1u);
-    }
-
-    // sums of probabilities
-    const int rows = 32 / call.lanes;  // of a warp at a time
-    const int lane_of_row = lane & (call.lanes - 1), row_of_warp = lane / call.lanes;
-    float sum[C * V];
+    if (lane == 0 && valid) atomicAdd(bins + experts, valid);
+    float column[S::E];
 #pragma unroll
-    for (int i = 0; i < C * V; ++i) sum[i] = 0.0f;
-    for (int64_t t = begin + warp * rows; t < end; t += kBalanceWarps * rows) {
-        const int64_t row = t + row_of_warp;
-        const bool there = row < end && (!call.mask || call.mask[row]);
-        RouterRow<T, V, C> r;
-        if (there) r.load(logits + row * call.logits_stride, call, lane_of_row);
-        float e[C * V], whole = 0.0f;
-        r.exponentials(e, call, lane_of_row, there);
+    for (int i = 0; i < S::E / 2; ++i) sum[i].apart(column[2 * i], column[2 * i + 1]);
 #pragma unroll
-        for (int i = 0; i < C * V; ++i) whole += e[i];
-        whole = row_sum(whole, call.lanes);
-        const float inverse = whole == 0.0f ? 0.0f : 1.0f / whole;
+    for (int i = 0; i < S::E; ++i)
 #pragma unroll
-        for (int i = 0; i < C * V; ++i) sum[i] = fmaf(e[i], inverse, sum[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < C * V; ++i)
-        for (int d = call.lanes; d < 32; d <<= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
+        for (int d = S::LANES; d < 32; d <<= 1) column[i] += __shfl_xor_sync(0xffffffffu, column[i], d);
     if (row_of_warp == 0) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int g = c * call.lanes + lane_of_row;
+        for (int c = 0; c < S::C; ++c) {
+            const int g = c * S::LANES + lane_of_row;
             if (g >= call.groups) continue;
 #pragma unroll
-            for (int v = 0; v < V; ++v) sums[warp * call.experts + g * V + v] = sum[c * V + v];
+            for (int v = 0; v < S::V; ++v) sums[warp * experts + g * S::V + v] = column[c * S::V + v];
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < call.experts; e += kBalanceThreads) {
-        float p = 0.0f;
+    for (int e = threadIdx.x; e <= experts; e += kBalanceThreads) {
+        if (e < experts) {
+            float p = sums[e];
 #pragma unroll
-        for (int w = 0; w < kBalanceWarps; ++w) p += sums[w * call.experts + e];
-        shares.sums[(int64_t)blockIdx.x * call.experts + e] = p;
+            for (int w = 1; w < kBalanceWarps; ++w) p += sums[w * experts + e];
+            if (alone) sums[e] = p;  // (this thread's own column)
+            else shares.sums[(int64_t)blockIdx.x * experts + e] = p;
+        }
+        if (!alone) shares.counts[(int64_t)blockIdx.x * (experts + 1) + e] = bins[e];
     }
-    for (int e = threadIdx.x; e <= call.experts; e += kBalanceThreads) shares.counts[(int64_t)blockIdx.x * (call.experts + 1) + e] = bins[e];
-    if (gridDim.x == 1) finish_balance(shares, 1, call.experts, call.choices, coefficient, loss, counts, probabilities);
+    if (!alone) return;
+    // One cluster has all tokens: it adds up by columns and needs no other launch.
+    cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = (int)cluster.num_blocks(), part = (experts + blocks - 1) / blocks, first = (int)cluster.block_rank() * part;
+    const int last = first + part < experts ? first + part : experts;
+    float *all_sums = sums + kBalanceWarps * padded_bins(experts);                   // [part]
+    unsigned int *all_counts = reinterpret_cast<unsigned int *>(all_sums + part);    // [part]
+    __shared__ unsigned int all_valid;
+    cluster.sync();
+    for (int e = first + threadIdx.x; e < last; e += kBalanceThreads) {
+        float p = 0.0f;
+        unsigned int n = 0u;
+        for (int b = 0; b < blocks; ++b) {
+            p += cluster.map_shared_rank(sums, b)[e];
+            n += cluster.map_shared_rank(bins, b)[e];
+        }
+        all_sums[e - first] = p;
+        all_counts[e - first] = n;
+    }
+    if (warp == kBalanceWarps - 1) {
+        const unsigned int n = __reduce_add_sync(0xffffffffu, lane < blocks ? cluster.map_shared_rank(bins, lane)[experts] : 0u);
+        if (lane == 0) all_valid = n;
+    }
+    cluster.sync();  // (nobody leaves while its shared memory is read)
+    finish_balance<kBalanceThreads>(all_sums, all_counts, first, last, all_valid, experts, to);
 }
 
-__global__ void __launch_bounds__(kBalanceThreads) balance_finish_kernel(BalanceShares shares, int blocks, int experts, int choices, double coefficient,
-                                                                          float *loss, int *counts, float *probabilities) {
+// The shares of all blocks, by a cluster whose blocks take a part of the columns each (444 blocks' shares added up by
+// the threads of one block took it 60 us).
+__global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(BalanceShares shares, int blocks, int experts, BalanceResult to) {
+    constexpr int kMostColumns = kMostExperts / kBalanceCluster;
+    __shared__ float sums[kMostColumns], part[kFinishThreads];
+    __shared__ unsigned int counts[kMostColumns], part_counts[kFinishThreads], valid[kFinishThreads / 32];
     grid_dependency_release();
+    const int columns = (experts + kBalanceCluster - 1) / kBalanceCluster, first = (int)blockIdx.x * columns;
+    const int last = first + columns < experts ? first + columns : experts;
+    // x threads along the columns, y along the shares
+    int x = 1;
+    while (x < columns) x *= 2;
+    const int y = kFinishThreads / x, tx = threadIdx.x & (x - 1), ty = threadIdx.x / x, e = first + tx;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    cg::this_cluster().sync();  // all its blocks run: they write to the first one's shared memory
     grid_dependency_wait();
-    finish_balance(shares, blocks, experts, choices, coefficient, loss, counts, probabilities);
+    const unsigned int some_valid = threadIdx.x < blocks ? shares.counts[threadIdx.x * (experts + 1) + experts] : 0u;
+    float p = 0.0f;
+    unsigned int n = 0u;
+    for (int b = ty; e < last && b < blocks; b += y * kShareAhead) {
+        float some[kShareAhead];
+        unsigned int count[kShareAhead];
+#pragma unroll
+        for (int u = 0; u < kShareAhead; ++u) {
+            const unsigned int at = b + u * y;  // (fewer than 2^20 values in all)
+            some[u] = at < blocks ? shares.sums[at * experts + e] : 0.0f;
+            count[u] = at < blocks ? shares.counts[at * (experts + 1) + e] : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kShareAhead; ++u) {
+            p += some[u];
+            n += count[u];
+        }
+    }
+    part[threadIdx.x] = p;
+    part_counts[threadIdx.x] = n;
+    n = __reduce_add_sync(0xffffffffu, some_valid);
+    if (lane == 0) valid[warp] = n;
+    __syncthreads();
+    for (int c = warp; c < columns; c += kFinishThreads / 32) {  // a warp adds up a column
+        p = 0.0f;
+        n = 0u;
+        for (int i = lane; i < y; i += 32) {
+            p += part[i * x + c];
+            n += part_counts[i * x + c];
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) p += __shfl_down_sync(0xffffffffu, p, d);
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) {
+            sums[c] = p;
+            counts[c] = n;
+        }
+    }
+    const unsigned int all_valid = __reduce_add_sync(0xffffffffu, valid[lane]);
+    __syncthreads();
+    finish_balance<kFinishThreads>(sums, counts, first, last, all_valid, experts, to);
 }
 
-template <typename T, int V, int C>
-__global__ void __launch_bounds__(kBalanceThreads)
+template <typename T, typename S>
+__global__ void __launch_bounds__(kGradientWarps * 32)
 balance_gradient_kernel(BalanceCall call, const T *__restrict__ logits, const int *counts, const float *loss_gradient, double coefficient,
                         T *gradient, int64_t gradient_stride, int accumulate) {
     grid_dependency_release();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rows = 32 / call.lanes;
-    const int lane_of_row = lane & (call.lanes - 1), row_of_warp = lane / call.lanes;
-    float often[C * V];
+    const int lane_of_row = lane & (S::LANES - 1), row_of_warp = lane / S::LANES;
+    const unsigned int rows = (unsigned int)call.tokens, apart = gridDim.x * (kGradientWarps * S::ROWS);
+    Pair often[S::E / 2];
+    auto often_of = [&](int i) {  // of the lane's i-th element
+        const int g = i / S::V * S::LANES + lane_of_row;
+        return g < call.groups ? (float)counts[g * S::V + i % S::V] : 0.0f;
+    };
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int g = c * call.lanes + lane_of_row;
-#pragma unroll
-        for (int v = 0; v < V; ++v) often[c * V + v] = g < call.groups ? (float)counts[g * V + v] : 0.0f;
-    }
+    for (int i = 0; i < S::E / 2; ++i) often[i] = Pair(often_of(2 * i), often_of(2 * i + 1));
     const double tokens = counts[call.experts];
     const float factor = tokens > 0.0 ? (float)((double)*loss_gradient * coefficient * call.experts / call.choices / (tokens * tokens)) : 0.0f;
-    const int64_t step = (int64_t)gridDim.x * kBalanceWarps * rows;
-    for (int64_t t = ((int64_t)blockIdx.x * kBalanceWarps + warp) * rows; t < call.tokens; t += step) {
-        const int64_t row = t + row_of_warp;
-        const bool there = row < call.tokens && (!call.mask || call.mask[row]);
-        RouterRow<T, V, C> r;
-        if (there) r.load(logits + row * call.logits_stride, call, lane_of_row);
-        float e[C * V], whole = 0.0f, dot = 0.0f;
-        r.exponentials(e, call, lane_of_row, there);
+    for (unsigned int t = (blockIdx.x * kGradientWarps + warp) * S::ROWS; t < rows; t += apart * S::U) {
+        RouterRow<T, S> r[S::U];
+        bool there[S::U];
 #pragma unroll
-        for (int i = 0; i < C * V; ++i) {
-            whole += e[i];
-            dot = fmaf(e[i], often[i], dot);
+        for (int u = 0; u < S::U; ++u) {
+            const unsigned int row = t + u * apart + row_of_warp;
+            there[u] = row < rows && (!call.mask || call.mask[row]);
+            r[u].load(logits + row * call.logits_stride, there[u], call.groups, lane_of_row);
         }
-        whole = row_sum(whole, call.lanes);
-        dot = row_sum(dot, call.lanes);
-        const float inverse = whole == 0.0f ? 0.0f : 1.0f / whole;
-        dot *= inverse;
-        if (row >= call.tokens || (!there && accumulate)) continue;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int g = c * call.lanes + lane_of_row;
-            if (g >= call.groups) continue;
-            T *p = gradient + row * gradient_stride + (int64_t)g * V;
-            float y[V];
-            Group<T, V> o;
+        for (int u = 0; u < S::U; ++u) {
+            const unsigned int row = t + u * apart + row_of_warp;
+            Pair e[S::E / 2];
+            r[u].exponentials(e);
+            Pair whole = e[0], dots = e[0] * often[0];
 #pragma unroll
-            for (int v = 0; v < V; ++v) y[v] = there ? factor * (e[c * V + v] * inverse) * (often[c * V + v] - dot) : 0.0f;
-            if (accumulate) {
-                o.load(p);
-#pragma unroll
-                for (int v = 0; v < V; ++v) y[v] += o.get(v);
+            for (int i = 1; i < S::E / 2; ++i) {
+                whole = whole + e[i];
+                dots = fma(e[i], often[i], dots);
             }
-            o.set(y);
-            o.store(p);
+            const float inverse = inverse_of(row_sum<S::LANES>(sum_of(whole)));
+            const float dot = row_sum<S::LANES>(sum_of(dots)) * inverse;
+            if (row >= rows || (!there[u] && accumulate)) continue;
+            const Pair by(factor * inverse, factor * inverse), less(-dot, -dot);
+            float y[S::E];
+#pragma unroll
+            for (int i = 0; i < S::E / 2; ++i) (e[i] * (often[i] + less) * by).apart(y[2 * i], y[2 * i + 1]);
+            T *p = gradient + row * gradient_stride;
+#pragma unroll
+            for (int c = 0; c < S::C; ++c) {
+                const int g = c * S::LANES + lane_of_row;
+                if (g >= call.groups) continue;
+                float z[S::V];
+                Group<T, S::V> o;
+#pragma unroll
+                for (int v = 0; v < S::V; ++v) z[v] = there[u] ? y[c * S::V + v] : 0.0f;
+                if (accumulate) {
+                    o.load(p + g * S::V);
+#pragma unroll
+                    for (int v = 0; v < S::V; ++v) z[v] += o.get(v);
+                }
+                o.set(z);
+                o.store(p + g * S::V);
+            }
         }
     }
 }
 
-// Calls `call` with the element type, the elements of a group and the groups of a lane that fit the logits.
+// Calls `call` with the element type and the shape of a row.  A lane holds about 16 elements of a row where the row is
+// that long, so that few lanes share a row and few shuffles go into its maximum and its sum.
 template <typename Call> static int with_row(int dtype, int experts, bool whole_groups, Call call) {
     return with_element(dtype, [&](auto element) {
         using T = decltype(element);
-        constexpr int V = 16 / sizeof(T);
-        const int lane_groups = (int)ceil_div(whole_groups ? experts / V : experts, 32);
+        constexpr int V = 16 / sizeof(T), C = 4;
         if (whole_groups) {
-            if (lane_groups <= 1) return call(element, std::integral_constant<int, V>{}, std::integral_constant<int, 1>{});
-            if (lane_groups <= 2) return call(element, std::integral_constant<int, V>{}, std::integral_constant<int, 2>{});
-            if constexpr (V == 8) {
-                return call(element, std::integral_constant<int, V>{}, std::integral_constant<int, 4>{});
-            } else {
-                if (lane_groups <= 4) return call(element, std::integral_constant<int, V>{}, std::integral_constant<int, 4>{});
-                return call(element, std::integral_constant<int, V>{}, std::integral_constant<int, 8>{});
-            }
+            const int groups = experts / V;
+            if (groups <= 2) return call(element, RowShape<V, 1, 2, 4>{});
+            if (groups <= 8) return call(element, RowShape<V, 2, 4, 2>{});
+            if (groups <= 16) return call(element, RowShape<V, C, 4, 1>{});
+            if (groups <= 32) return call(element, RowShape<V, C, 8, 1>{});
+            if (groups <= 64) return call(element, RowShape<V, C, 16, 1>{});
+            if (groups <= 128) return call(element, RowShape<V, C, 32, 1>{});
+            if constexpr (V == 4) return call(element, RowShape<V, 2 * C, 32, 1>{});
+            return (int)B200ALG_UNSUPPORTED;  // (no type has more: 1024 experts are the most)
         }
-        if (lane_groups <= 2) return call(element, std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
-        if (lane_groups <= 8) return call(element, std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
-        return call(element, std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+        if (experts <= 16) return call(element, RowShape<1, 8, 2, 2>{});
+        if (experts <= 64) return call(element, RowShape<1, 8, 8, 2>{});
+        if (experts <= 256) return call(element, RowShape<1, 8, 32, 2>{});
+        return call(element, RowShape<1, 32, 32, 1>{});
     });
 }
 
-static BalanceCall balance_call(int64_t tokens, int64_t logits_stride, int64_t experts, int64_t choices, const void *mask, int group) {
-    BalanceCall c{tokens, logits_stride, (int)experts, (int)choices, (const unsigned char *)mask, 1, (int)experts / group};
-    while (c.lanes < 32 && c.lanes < c.groups) c.lanes *= 2;
-    return c;
+template <typename S> static BalanceCall balance_call(int64_t tokens, int64_t logits_stride, int64_t experts, int64_t choices, const void *mask) {
+    return BalanceCall{tokens, logits_stride, (int)experts, (int)choices, (const unsigned char *)mask, (int)experts / S::V};
 }
 
-// Blocks that a call's tokens fill: every warp has a few rows.
-static int64_t balance_blocks(int64_t tokens, int64_t most) {
-    const int64_t want = ceil_div(tokens, kBalanceWarps * 8);
-    return want < 1 ? 1 : want < most ? want : most;
+// Blocks of a call: one for a few rows, then a cluster of them, and from about a megabyte on (0) as many as there is
+// work for.
+static int balance_cluster(int64_t tokens, int64_t experts) {
+    const int64_t cells = tokens * experts;
+    return cells <= 4096 ? 1 : cells <= 1 << 18 ? kBalanceCluster : 0;
+}
+
+// Resident blocks of a kernel on the whole GPU (asked once per context; `cache` is the kernel's own).
+template <typename KernelT> static int resident_blocks(KernelT kernel, int threads, size_t smem, ContextCache<int> &cache, int *blocks) {
+    int per_sm = 0;
+    if (!cache.find(&per_sm)) {
+        if (smem > 48 << 10) B200ALG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        B200ALG_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+        if (per_sm < 1) per_sm = 1;
+        cache.store(per_sm);
+    }
+    *blocks = sm_count() * per_sm;
+    return B200ALG_OK;
 }
 
 static int check_router(int64_t tokens, int64_t experts, int64_t choices, int64_t logits_stride, int dtype) {
@@ -293,7 +529,7 @@ static int check_router(int64_t tokens, int64_t experts, int64_t choices, int64_
 }
 
 static int64_t balance_temp_bytes(int64_t experts, int64_t tokens) {
-    const int64_t blocks = balance_blocks(tokens, kMostBalanceBlocks);
+    const int64_t blocks = balance_cluster(tokens, experts) ? 0 : kMostBalanceBlocks;
     return sizeof(TempHeader) + round_up(blocks * experts * 4, 256) + round_up(blocks * (experts + 1) * 4, 256);
 }
 
@@ -323,24 +559,36 @@ extern "C" int b200alg_balance_loss(void *stream, const void *logits, int64_t to
         return B200ALG_MISALIGNED;
     if (temp_bytes < balance_temp_bytes(experts, tokens)) return B200ALG_TEMP_TOO_SMALL;
     cudaStream_t s = (cudaStream_t)stream;
-    const int64_t resident = (int64_t)sm_count() * kBalanceBlocksPerSm;
-    const int blocks = (int)balance_blocks(tokens, resident < kMostBalanceBlocks ? resident : kMostBalanceBlocks);
+    const int cluster = balance_cluster(tokens, experts);
+    int blocks = 0;
     BalanceShares shares;
     shares.sums = (float *)((char *)temp + sizeof(TempHeader));
-    shares.counts = (unsigned int *)((char *)temp + sizeof(TempHeader) + round_up((int64_t)blocks * experts * 4, 256));
+    shares.counts = (unsigned int *)((char *)temp + sizeof(TempHeader) + round_up(kMostBalanceBlocks * experts * 4, 256));
+    const BalanceResult to{coefficient * experts / choices, loss, counts, probabilities};
     const bool whole = groups_aligned(logits, logits_stride, tokens, experts, bytes, 16 / bytes);
-    const size_t smem = (size_t)(padded_bins((int)experts) + kBalanceWarps * experts) * 4;
-    rc = with_row(dtype, (int)experts, whole, [&](auto element, auto v, auto c) -> int {
+    const size_t smem = (size_t)padded_bins((int)experts) * (1 + kBalanceWarps) * 4 + (cluster ? (size_t)ceil_div(experts, cluster) * 8 : 0);
+    rc = with_row(dtype, (int)experts, whole, [&](auto element, auto shape) -> int {
         using T = decltype(element);
-        const BalanceCall call = balance_call(tokens, logits_stride, experts, choices, mask, v.value);
-        B200ALG_CUDA_TRY(launch_dependent(balance_kernel<T, v.value, c.value>, dim3(blocks), dim3(kBalanceThreads), smem, s, call, (const T *)logits,
-                                          IndexView{chosen, chosen_stride, chosen_dtype == B200ALG_I64}, FastDivide((unsigned int)choices), shares,
-                                          coefficient, loss, counts, probabilities));
+        using S = decltype(shape);
+        auto kernel = balance_kernel<T, S>;
+        static ContextCache<int> cache;
+        const int status = resident_blocks(kernel, kBalanceThreads, kBalanceSmem, cache, &blocks);
+        if (status != B200ALG_OK) return status;
+        if (cluster) {
+            blocks = cluster;
+        } else {
+            const int64_t want = ceil_div(tokens, kBalanceWarps * S::ROWS * S::U);
+            if (blocks > kMostBalanceBlocks) blocks = kMostBalanceBlocks;
+            if (blocks > want) blocks = (int)want;
+        }
+        B200ALG_CUDA_TRY(launch_dependent_cluster(kernel, dim3(blocks), dim3(kBalanceThreads), smem, s, cluster ? cluster : 1,
+                                                  balance_call<S>(tokens, logits_stride, experts, choices, mask), (const T *)logits,
+                                                  IndexView{chosen, chosen_stride, chosen_dtype == B200ALG_I64}, shares, to, cluster != 0));
         return B200ALG_OK;
     });
-    if (rc != B200ALG_OK || blocks == 1) return rc;
-    B200ALG_CUDA_TRY(launch_dependent(balance_finish_kernel, dim3(1), dim3(kBalanceThreads), 0, s, shares, blocks, (int)experts, (int)choices,
-                                      coefficient, loss, counts, probabilities));
+    if (rc != B200ALG_OK || cluster) return rc;
+    B200ALG_CUDA_TRY(launch_dependent_cluster(balance_finish_kernel, dim3(kBalanceCluster), dim3(kFinishThreads), 0, s, kBalanceCluster, shares, blocks,
+                                              (int)experts, to));
     return B200ALG_OK;
 }
 
@@ -357,13 +605,18 @@ extern "C" int b200alg_balance_loss_gradient(void *stream, const void *logits, i
     cudaStream_t s = (cudaStream_t)stream;
     const bool whole = groups_aligned(logits, logits_stride, tokens, experts, bytes, 16 / bytes) &&
                        groups_aligned(gradient, gradient_stride, tokens, experts, bytes, 16 / bytes);
-    return with_row(dtype, (int)experts, whole, [&](auto element, auto v, auto c) -> int {
+    return with_row(dtype, (int)experts, whole, [&](auto element, auto shape) -> int {
         using T = decltype(element);
-        const BalanceCall call = balance_call(tokens, logits_stride, experts, choices, mask, v.value);
-        const int64_t want = ceil_div(tokens, (32 / call.lanes) * kBalanceWarps), most = (int64_t)sm_count() * 8;
-        B200ALG_CUDA_TRY(launch_dependent(balance_gradient_kernel<T, v.value, c.value>, dim3((unsigned)(want < most ? want : most)),
-                                          dim3(kBalanceThreads), 0, s, call, (const T *)logits, counts, loss_gradient, coefficient, (T *)gradient,
-                                          gradient_stride, accumulate != 0));
+        using S = decltype(shape);
+        auto kernel = balance_gradient_kernel<T, S>;
+        int blocks = 0;
+        static ContextCache<int> cache;
+        const int status = resident_blocks(kernel, kGradientWarps * 32, 0, cache, &blocks);
+        if (status != B200ALG_OK) return status;
+        const int64_t want = ceil_div(tokens, kGradientWarps * S::ROWS * S::U);
+        B200ALG_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)(want < blocks ? want : blocks)), dim3(kGradientWarps * 32), 0, s,
+                                          balance_call<S>(tokens, logits_stride, experts, choices, mask), (const T *)logits, counts, loss_gradient,
+                                          coefficient, (T *)gradient, gradient_stride, accumulate != 0));
         return B200ALG_OK;
     });
 }

@@ -180,7 +180,7 @@ def test_refusals(accelerator):
         (dict(logits=None), ib.ArgumentNullException), (dict(logits=logits.double()), ib.NotSupportedException), (dict(logits=logits[0]), ib.ArgumentOutOfRangeException),
         (dict(experts=chosen.float()), ib.NotSupportedException), (dict(experts=chosen[:5]), ib.ArgumentOutOfRangeException), (dict(mask=mask[:5]), ib.ArgumentOutOfRangeException),
         (dict(mask=mask.float()), ib.InvalidOperationException), (dict(counts=counts[:8]), ib.ArgumentOutOfRangeException), (dict(counts=counts.long()), ib.InvalidOperationException),
-        (dict(probabilities=p[:7]), ib.ArgumentOutOfRangeException), (dict(loss=loss[:0]), ib.ArgumentOutOfRangeException), (dict(temp=temp[:64]), ib.ArgumentOutOfRangeException),
+        (dict(probabilities=p[:7]), ib.ArgumentOutOfRangeException), (dict(loss=loss[:0]), ib.ArgumentOutOfRangeException), (dict(temp=temp[:-1]), ib.ArgumentOutOfRangeException),
         (dict(experts=chosen.cpu()), ib.InvalidOperationException), (dict(experts=chosen[:, :0]), ib.B200AlgException),
         (dict(logits=torch.zeros(6, 1_025, device="cuda"), counts=counts.new_zeros(1_026), probabilities=p.new_zeros(1_025)), ib.NotSupportedException),
     ]:
