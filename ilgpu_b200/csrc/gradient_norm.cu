@@ -12,10 +12,13 @@
 namespace b200alg {
 
 constexpr int kNormThreads = 256;
-constexpr int kChunk = 8192;       // elements
+constexpr int kGroupBytes = 16;
+constexpr int kAheadGroups = 4;                                          // of a thread in a chunk
+constexpr int kChunkGroups = kNormThreads * kAheadGroups;                // 16 KB
 constexpr int kNormBlocksPerSm = 4;
 constexpr int kMaxBlocks = 148 * kNormBlocksPerSm;  // partial sums of a launch
-constexpr int kMostViews = 1024;   // of a launch: 30 KB of parameters
+constexpr int kMostViews = 1024;                    // of a launch: 30 KB of parameters
+constexpr int kMostSpan = 8;                        // chunks that a block takes one behind the other
 
 struct ViewTable {
     const void *in[kMostViews];
@@ -24,8 +27,14 @@ struct ViewTable {
     unsigned int chunk[kMostViews + 1];  // first chunk of a view
     unsigned char in_type[kMostViews], out_type[kMostViews];
     int views;
+    int span;
 };
 static_assert(sizeof(ViewTable) <= 31 << 10, "fits a kernel's parameters");
+
+// 16-byte groups of a view, from the boundary at or in front of its first element on.
+__host__ __device__ __forceinline__ int64_t groups_of(const void *p, int64_t length, int bytes) {
+    return ((int64_t)((uintptr_t)p & (kGroupBytes - 1)) + length * bytes + kGroupBytes - 1) / kGroupBytes;
+}
 
 // Views from `first` on that one launch takes; returns how many.
 static int64_t fill_table(ViewTable &t, const void *const *in, void *const *out, const int64_t *lengths, const int *in_types, const int *out_types,
@@ -34,8 +43,7 @@ static int64_t fill_table(ViewTable &t, const void *const *in, void *const *out,
     unsigned int chunks = 0;
     t.views = 0;
     for (; i < views && t.views < kMostViews; ++i) {
-        const int64_t need = ceil_div(lengths[i], kChunk);
-        if (!need) continue;
+        if (!lengths[i]) continue;
         const int v = t.views++;
         t.in[v] = in[i];
         t.out[v] = out ? out[i] : (void *)in[i];
@@ -43,190 +51,253 @@ static int64_t fill_table(ViewTable &t, const void *const *in, void *const *out,
         t.chunk[v] = chunks;
         t.in_type[v] = (unsigned char)in_types[i];
         t.out_type[v] = (unsigned char)(out_types ? out_types[i] : in_types[i]);
-        chunks += (unsigned int)need;
+        chunks += (unsigned int)ceil_div(groups_of(in[i], lengths[i], element_bytes(in_types[i])), kChunkGroups);
     }
     t.chunk[t.views] = chunks;
+    const int64_t each = chunks / ((int64_t)kMaxBlocks * 4);
+    t.span = (int)(each < 1 ? 1 : each > kMostSpan ? kMostSpan : each);
     return i - first;
 }
 
-// The view that chunk c belongs to.
-__device__ __forceinline__ int view_of_chunk(const ViewTable &t, unsigned int c) {
-    int lo = 0, hi = t.views - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.chunk[mid] <= c) lo = mid;
-        else hi = mid - 1;
+// The chunks of a block: spans of a few one behind the other, taken in turn by all blocks, so that all of them read the
+// same part of memory at a time (a stretch of its own for each block: 5.4 TB/s instead of XX).  LAST_FIRST: from the end on.
+template <bool LAST_FIRST> struct Chunks {
+    const ViewTable &t;
+    unsigned int span, chunk, left;  // left: chunks of the span behind this one
+    int view;
+    __device__ __forceinline__ Chunks(const ViewTable &table) : t(table), span(blockIdx.x) {}
+    __device__ __forceinline__ unsigned int spans() const { return (t.chunk[t.views] + t.span - 1) / t.span; }
+    __device__ __forceinline__ bool enter() {
+        if (span >= spans()) return false;
+        const unsigned int at = LAST_FIRST ? spans() - 1 - span : span, begin = at * t.span, behind = begin + t.span;
+        const unsigned int end = behind < t.chunk[t.views] ? behind : t.chunk[t.views];
+        left = end - begin - 1;
+        chunk = LAST_FIRST ? end - 1 : begin;
+        int lo = 0, hi = t.views - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (t.chunk[mid] <= chunk) lo = mid;
+            else hi = mid - 1;
+        }
+        view = lo;
+        return true;
     }
-    return lo;
+    __device__ __forceinline__ bool next() {
+        if (!left) {
+            span += gridDim.x;
+            return enter();
+        }
+        --left;
+        if (LAST_FIRST) {
+            --chunk;
+            while (chunk < t.chunk[view]) --view;
+        } else {
+            ++chunk;
+            while (chunk >= t.chunk[view + 1]) ++view;
+        }
+        return true;
+    }
+};
+
+// A thread's part of a chunk: kAheadGroups groups, zero where the view has none.
+struct Part {
+    uint4 w[kAheadGroups];
+    int type, view;
+    int64_t group;  // of the view, the thread's first
+};
+
+template <typename T> __device__ __forceinline__ uint4 edge_group(const T *in, int64_t first, int64_t length) {
+    Group<T, kGroupBytes / (int)sizeof(T)> g;
+    g.clear();
+#pragma unroll
+    for (int k = 0; k < kGroupBytes / (int)sizeof(T); ++k) {
+        if (first + k < 0 || first + k >= length) continue;
+        if constexpr (sizeof(T) == 4) g.w[k] = reinterpret_cast<const unsigned int *>(in)[first + k];
+        else g.w[k / 2] |= (unsigned int)reinterpret_cast<const unsigned short *>(in)[first + k] << (k % 2 * 16);
+    }
+    return make_uint4(g.w[0], g.w[1], g.w[2], g.w[3]);
 }
 
-// A block's stretch of the chunks.
-__device__ __forceinline__ void stretch(unsigned int chunks, unsigned int &begin, unsigned int &end) {
-    begin = (unsigned int)((unsigned long long)chunks * blockIdx.x / gridDim.x);
-    end = (unsigned int)((unsigned long long)chunks * (blockIdx.x + 1) / gridDim.x);
+// Loads this thread's part of the chunk; LAST: the data is not needed again.
+template <typename Where> __device__ __forceinline__ void load_part(Part &part, const ViewTable &t, const Where &at) {
+    const int v = at.view;
+    part.view = v;
+    part.type = t.in_type[v];
+    const int shift = part.type == B200ALG_F32 ? 2 : 1;  // of an element's size
+    const int before = (int)((uintptr_t)t.in[v] & (kGroupBytes - 1));  // bytes of the first group in front of the view
+    const char *base = (const char *)t.in[v] - before;
+    const int64_t bytes = (t.length[v] << shift) + before;
+    part.group = (int64_t)(at.chunk - t.chunk[v]) * kChunkGroups + threadIdx.x;
+    const int64_t whole = bytes / kGroupBytes;  // groups in front of this one are full, but for the first where `before`
+#pragma unroll
+    for (int u = 0; u < kAheadGroups; ++u) {
+        const int64_t g = part.group + u * kNormThreads;
+        if (g < whole && (g || !before)) {
+            part.w[u] = __ldcs(reinterpret_cast<const uint4 *>(base) + g);
+        } else if (g * kGroupBytes < bytes) {
+            const int64_t first = (g * kGroupBytes - before) >> shift;
+            part.w[u] = shift == 2 ? edge_group((const float *)t.in[v], first, t.length[v]) : edge_group((const __half *)t.in[v], first, t.length[v]);
+        } else {
+            part.w[u] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
 }
 
-// Squares of G elements in 32 bits; where they overflow or vanish there, in 64.
-template <typename T, int G, int N> __device__ __forceinline__ double squares(const Group<T, G> (&v)[N]) {
+// Squares of a part in 32 bits; where they overflow or vanish there, in 64.
+template <typename T> __device__ __forceinline__ double squares(const Part &part) {
+    constexpr int G = kGroupBytes / (int)sizeof(T);
     float s = 0.0f;
     unsigned int any = 0u;
+    auto group = [&](int u) {
+        Group<T, G> g;
+        g.w[0] = part.w[u].x, g.w[1] = part.w[u].y, g.w[2] = part.w[u].z, g.w[3] = part.w[u].w;
+        return g;
+    };
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
+    for (int u = 0; u < kAheadGroups; ++u) {
+        const Group<T, G> g = group(u);
+        float sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < G; ++k) s = fmaf(v[u].get(k), v[u].get(k), s);
-        if constexpr (!std::is_same<T, __half>::value) {
-#pragma unroll
-            for (int k = 0; k < Group<T, G>::kWords; ++k) any |= v[u].w[k];
-        }
+        for (int k = 0; k < G; ++k) sum = fmaf(g.get(k), g.get(k), sum);
+        s += sum;
+        any |= g.w[0] | g.w[1] | g.w[2] | g.w[3];
     }
     if constexpr (!std::is_same<T, __half>::value) {  // (the squares of 16-bit floats of five exponent bits are all normal)
         constexpr unsigned int kMagnitude = sizeof(T) == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
-        // Squares below 2^-126 lose bits, each at most 2^-126; N * G of them are nothing beside 2^-80.
+        // Squares below 2^-126 lose bits, each at most 2^-126; 32 of them are nothing beside 2^-80.
         if (!(s >= 0x1p-80f && s <= FLT_MAX) && (any & kMagnitude)) {
             double d = 0.0;
 #pragma unroll
-            for (int u = 0; u < N; ++u)
+            for (int u = 0; u < kAheadGroups; ++u) {
+                const Group<T, G> g = group(u);
 #pragma unroll
-                for (int k = 0; k < G; ++k) d = fma((double)v[u].get(k), (double)v[u].get(k), d);
+                for (int k = 0; k < G; ++k) d = ::fma((double)g.get(k), (double)g.get(k), d);
+            }
             return d;
         }
     }
     return (double)s;
 }
 
-// Sum of the squares of a chunk, this thread's part.
-template <typename T> __device__ __forceinline__ double chunk_squares(const T *__restrict__ p, int64_t n) {
-    constexpr int G = 16 / sizeof(T);
-    constexpr int N = kChunk / (kNormThreads * G);
-    double sum = 0.0;
-    int64_t head = (int64_t)(((16u - (unsigned)((uintptr_t)p & 15u)) & 15u) / sizeof(T));
-    if (head > n) head = n;
-    const int64_t groups = (n - head) / G;
-    Group<T, G> v[N];
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-        const int64_t g = threadIdx.x + u * kNormThreads;
-        if (g < groups) v[u].load(p + head + g * G);
-        else v[u].clear();
-    }
-    sum = squares<T, G, N>(v);
-    const int64_t tail = head + groups * G;
-    const int64_t at = (int64_t)threadIdx.x < head ? (int64_t)threadIdx.x : tail + threadIdx.x - head;  // fewer than 32 elements
-    if (at < n && (int64_t)threadIdx.x < head + n - tail) {
-        Group<T, 1> one[1];
-        one[0].load(p + at);
-        sum += squares<T, 1, 1>(one);
-    }
-    return sum;
-}
-
-// Sum over the block, in its first thread.
+// Sum over the block, in every thread.
 __device__ __forceinline__ double block_sum(double v) {
     __shared__ double part[kNormThreads / 32];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_down_sync(0xffffffffu, v, d);
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        v = part[0];
-        for (int i = 1; i < kNormThreads / 32; ++i) v += part[i];
-    }
-    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int i = 1; i < kNormThreads / 32; ++i) v += part[i];
     return v;
+}
+
+// The norm from the sums of all blocks, added up in a fixed order.
+__device__ __forceinline__ float norm_of(const double *partial, int count) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < count; i += kNormThreads) sum += partial[i];
+    return (float)sqrt(block_sum(sum));
 }
 
 __global__ void __launch_bounds__(kNormThreads) norm_partial_kernel(const __grid_constant__ ViewTable t, double *partial) {
     grid_dependency_release();
+    Chunks<false> at(t);
+    bool more = at.enter();
     grid_dependency_wait();
-    unsigned int c, end;
-    stretch(t.chunk[t.views], c, end);
     double sum = 0.0;
-    if (c < end) {
-        int v = view_of_chunk(t, c);
-        for (; c < end; ++c) {
-            while (c >= t.chunk[v + 1]) ++v;
-            const int64_t first = (int64_t)(c - t.chunk[v]) * kChunk;
-            const int64_t n = t.length[v] - first < kChunk ? t.length[v] - first : kChunk;
-            switch (t.in_type[v]) {
-            case B200ALG_F32: sum += chunk_squares((const float *)t.in[v] + first, n); break;
-            case B200ALG_F16: sum += chunk_squares((const __half *)t.in[v] + first, n); break;
-            case B200ALG_BF16: sum += chunk_squares((const __nv_bfloat16 *)t.in[v] + first, n); break;
-            }
+    Part next;
+    if (more) load_part(next, t, at);
+    while (more) {  // the next chunk is under way while this one is added up
+        const Part part = next;
+        more = at.next();
+        if (more) load_part(next, t, at);
+        switch (part.type) {
+        case B200ALG_F32: sum += squares<float>(part); break;
+        case B200ALG_F16: sum += squares<__half>(part); break;
+        default: sum += squares<__nv_bfloat16>(part);
         }
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// The partial sums are added up in a fixed order.
-__global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(const double *partial, int64_t count, float *norm) {
+__global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(const double *partial, int count, float *norm) {
     grid_dependency_release();
     grid_dependency_wait();
-    double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < count; i += kNormThreads) sum += partial[i];
-    sum = block_sum(sum);
-    if (threadIdx.x == 0) *norm = (float)sqrt(sum);
+    const float whole = norm_of(partial, count);
+    if (threadIdx.x == 0) *norm = whole;
 }
 
-template <typename TIn, typename TOut>
-__device__ __forceinline__ void scale_chunk(const TIn *in, TOut *out, int64_t n, float factor) {
-    constexpr int G = 16 / sizeof(TIn);
-    // groups where both sides can be moved whole: from the input's first boundary on
-    int64_t head = (int64_t)(((16u - (unsigned)((uintptr_t)in & 15u)) & 15u) / sizeof(TIn));
+template <typename TIn, typename TOut> __device__ __forceinline__ void scale_part(const Part &part, const ViewTable &t, float factor) {
+    constexpr int G = kGroupBytes / (int)sizeof(TIn);
     constexpr unsigned int kBoundary = G * sizeof(TOut) < 16 ? G * sizeof(TOut) : 16;
-    if (head > n || (uintptr_t)(out + head) % kBoundary) head = n;
-    const int64_t groups = (n - head) / G, tail = head + groups * G;
-    for (int64_t g = threadIdx.x; g < groups; g += kNormThreads) {
-        Group<TIn, G> v;
-        v.load(in + head + g * G);
+    const int64_t length = t.length[part.view];
+    const int before = (int)((uintptr_t)t.in[part.view] & (kGroupBytes - 1)) / (int)sizeof(TIn);
+#pragma unroll
+    for (int u = 0; u < kAheadGroups; ++u) {
+        const int64_t first = (part.group + u * kNormThreads) * G - before;  // the group's first element
+        if (first >= length) continue;
+        TOut *to = (TOut *)t.out[part.view] + first;
+        Group<TIn, G> g;
+        g.w[0] = part.w[u].x, g.w[1] = part.w[u].y, g.w[2] = part.w[u].z, g.w[3] = part.w[u].w;
         float x[G];
 #pragma unroll
-        for (int k = 0; k < G; ++k) x[k] = v.get(k) * factor;
-        Group<TOut, G> y;
-        y.set(x);
-        y.store(out + head + g * G);
-    }
-    for (int64_t i = threadIdx.x; i < head; i += kNormThreads) out[i] = from_float<TOut>(to_float(in[i]) * factor);
-    for (int64_t i = tail + threadIdx.x; i < n; i += kNormThreads) out[i] = from_float<TOut>(to_float(in[i]) * factor);
-}
-
-template <typename TIn>
-__device__ __forceinline__ void scale_chunk_to(const TIn *in, void *out, int out_type, int64_t first, int64_t n, float factor) {
-    switch (out_type) {
-    case B200ALG_F32: scale_chunk(in + first, (float *)out + first, n, factor); break;
-    case B200ALG_F16: scale_chunk(in + first, (__half *)out + first, n, factor); break;
-    case B200ALG_BF16: scale_chunk(in + first, (__nv_bfloat16 *)out + first, n, factor); break;
+        for (int k = 0; k < G; ++k) x[k] = g.get(k) * factor;
+        if (first >= 0 && first + G <= length && (uintptr_t)to % kBoundary == 0) {
+            Group<TOut, G> y;
+            y.set(x);
+            y.store(to);
+        } else {
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+                if (first + k >= 0 && first + k < length) to[k] = from_float<TOut>(x[k]);
+        }
     }
 }
 
-__global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_constant__ ViewTable t, const float *norm, double max_norm) {
+template <typename TIn> __device__ __forceinline__ void scale_part_from(const Part &part, const ViewTable &t, float factor) {
+    switch (t.out_type[part.view]) {
+    case B200ALG_F32: scale_part<TIn, float>(part, t, factor); break;
+    case B200ALG_F16: scale_part<TIn, __half>(part, t, factor); break;
+    default: scale_part<TIn, __nv_bfloat16>(part, t, factor);
+    }
+}
+
+// partial == NULL: by the norm that is there; else the norm comes from the blocks' sums, and the first block stores it.
+// (Every block adds them up itself, so that no launch stands between the two passes.)
+__global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_constant__ ViewTable t, const double *partial, int count, float *norm, double max_norm) {
     grid_dependency_release();
+    Chunks<true> at(t);  // backwards: what the norm's pass has read last may still be in the cache
+    bool more = at.enter();
     grid_dependency_wait();
-    const float whole = *norm;
+    Part next;
+    if (more) load_part(next, t, at);
+    float whole;
+    if (partial) {
+        whole = norm_of(partial, count);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *norm = whole;
+    } else {
+        whole = *norm;
+    }
     // a norm that is not finite leaves the values as they are: it says so itself
     const float factor = whole <= FLT_MAX && (double)whole > max_norm ? (float)(max_norm / (double)whole) : 1.0f;
-    unsigned int begin, c;
-    stretch(t.chunk[t.views], begin, c);
-    if (c <= begin) return;
-    int v = view_of_chunk(t, c - 1);
-    // backwards: what the norm's kernel has read last may still be in the cache
-    while (c-- > begin) {
-        while (c < t.chunk[v]) --v;
-        if (factor == 1.0f && t.in[v] == t.out[v]) continue;
-        const int64_t first = (int64_t)(c - t.chunk[v]) * kChunk;
-        const int64_t n = t.length[v] - first < kChunk ? t.length[v] - first : kChunk;
-        switch (t.in_type[v]) {
-        case B200ALG_F32: scale_chunk_to((const float *)t.in[v], t.out[v], t.out_type[v], first, n, factor); break;
-        case B200ALG_F16: scale_chunk_to((const __half *)t.in[v], t.out[v], t.out_type[v], first, n, factor); break;
-        case B200ALG_BF16: scale_chunk_to((const __nv_bfloat16 *)t.in[v], t.out[v], t.out_type[v], first, n, factor); break;
+    while (more) {
+        const Part part = next;
+        more = at.next();
+        if (more) load_part(next, t, at);
+        if (factor == 1.0f && t.in[part.view] == t.out[part.view]) continue;
+        switch (part.type) {
+        case B200ALG_F32: scale_part_from<float>(part, t, factor); break;
+        case B200ALG_F16: scale_part_from<__half>(part, t, factor); break;
+        default: scale_part_from<__nv_bfloat16>(part, t, factor);
         }
     }
 }
 
 static int blocks_of(const ViewTable &t) {
     const int64_t most = kMaxBlocks < (int64_t)sm_count() * kNormBlocksPerSm ? kMaxBlocks : (int64_t)sm_count() * kNormBlocksPerSm;
-    const int64_t chunks = t.chunk[t.views];
-    return (int)(chunks < most ? chunks : most);
+    const int64_t spans = ceil_div(t.chunk[t.views], t.span);
+    return (int)(spans < most ? spans : most);
 }
 
 // launch_dependent() without its copies of the parameters.
@@ -266,31 +337,38 @@ static int64_t norm_temp_bytes(int64_t count) {
     return sizeof(TempHeader) + round_up((ceil_div(count, kMostViews) + 1) * kMaxBlocks * 8, 256);  // every launch but the last takes kMostViews views
 }
 
-static int run_norm(cudaStream_t s, const void *const *views, const int64_t *lengths, const int *types, int64_t count, float *norm, void *temp) {
+// The sums of squares of all launches' blocks; *sums: how many there are.
+static int run_partial(cudaStream_t s, const void *const *views, const int64_t *lengths, const int *types, int64_t count, void *temp, int *sums) {
     double *partial = (double *)((char *)temp + sizeof(TempHeader));
-    int64_t sums = 0;
+    *sums = 0;
     ViewTable t;
     for (int64_t first = 0; first < count;) {
         first += fill_table(t, views, nullptr, lengths, types, nullptr, first, count);
         if (!t.views) break;
         const int blocks = blocks_of(t);
-        double *to = partial + sums;
+        double *to = partial + *sums;
         void *arguments[] = {&t, &to};
         B200ALG_CUDA_TRY(launch_with_table((const void *)norm_partial_kernel, blocks, s, arguments));
-        sums += blocks;
+        *sums += blocks;
     }
-    B200ALG_CUDA_TRY(launch_dependent(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, (const double *)partial, sums, norm));
     return B200ALG_OK;
 }
 
+static int run_finish(cudaStream_t s, int sums, float *norm, void *temp) {
+    B200ALG_CUDA_TRY(launch_dependent(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, (const double *)((char *)temp + sizeof(TempHeader)), sums, norm));
+    return B200ALG_OK;
+}
+
+// By the norm that is there (partial == NULL), or by that of `sums` partial sums, which the first launch stores.
 static int run_scale(cudaStream_t s, const void *const *views, void *const *outputs, const int64_t *lengths, const int *types, const int *out_types,
-                     int64_t count, const float *norm, double max_norm) {
+                     int64_t count, const double *partial, int sums, float *norm, double max_norm) {
     ViewTable t;
     for (int64_t first = 0; first < count;) {
         first += fill_table(t, views, outputs, lengths, types, out_types, first, count);
         if (!t.views) break;
-        void *arguments[] = {&t, &norm, &max_norm};
+        void *arguments[] = {&t, &partial, &sums, &norm, &max_norm};
         B200ALG_CUDA_TRY(launch_with_table((const void *)scale_kernel, blocks_of(t), s, arguments));
+        partial = nullptr;  // the norm is there now
     }
     return B200ALG_OK;
 }
@@ -313,7 +391,9 @@ extern "C" int b200alg_gradient_norm(void *stream, const void *const *views, con
     if (!norm || !temp) return B200ALG_INVALID_ARGUMENT;
     if ((uintptr_t)norm % 4 || (uintptr_t)temp % 256) return B200ALG_MISALIGNED;
     if (temp_bytes < norm_temp_bytes(count)) return B200ALG_TEMP_TOO_SMALL;
-    return run_norm((cudaStream_t)stream, views, lengths, dtypes, count, norm, temp);
+    int sums = 0;
+    const int status = run_partial((cudaStream_t)stream, views, lengths, dtypes, count, temp, &sums);
+    return status != B200ALG_OK ? status : run_finish((cudaStream_t)stream, sums, norm, temp);
 }
 
 extern "C" int b200alg_gradient_scale(void *stream, const void *const *views, void *const *outputs, const int64_t *lengths, const int *dtypes,
@@ -322,7 +402,7 @@ extern "C" int b200alg_gradient_scale(void *stream, const void *const *views, vo
     if (rc != B200ALG_OK) return rc;
     if (!norm || !(max_norm >= 0.0)) return B200ALG_INVALID_ARGUMENT;
     if ((uintptr_t)norm % 4) return B200ALG_MISALIGNED;
-    return run_scale((cudaStream_t)stream, views, outputs, lengths, dtypes, out_dtypes, count, norm, max_norm);
+    return run_scale((cudaStream_t)stream, views, outputs, lengths, dtypes, out_dtypes, count, nullptr, 0, (float *)norm, max_norm);
 }
 
 extern "C" int b200alg_gradient_clip(void *stream, const void *const *views, void *const *outputs, const int64_t *lengths, const int *dtypes,
@@ -332,7 +412,10 @@ extern "C" int b200alg_gradient_clip(void *stream, const void *const *views, voi
     if (!norm || !temp || !(max_norm >= 0.0)) return B200ALG_INVALID_ARGUMENT;
     if ((uintptr_t)norm % 4 || (uintptr_t)temp % 256) return B200ALG_MISALIGNED;
     if (temp_bytes < norm_temp_bytes(count)) return B200ALG_TEMP_TOO_SMALL;
-    rc = run_norm((cudaStream_t)stream, views, lengths, dtypes, count, norm, temp);
+    int sums = 0;
+    rc = run_partial((cudaStream_t)stream, views, lengths, dtypes, count, temp, &sums);
     if (rc != B200ALG_OK) return rc;
-    return run_scale((cudaStream_t)stream, views, outputs, lengths, dtypes, out_dtypes, count, norm, max_norm);
+    if (!sums) return run_finish((cudaStream_t)stream, sums, norm, temp);  // nothing to clip
+    return run_scale((cudaStream_t)stream, views, outputs, lengths, dtypes, out_dtypes, count, (const double *)((char *)temp + sizeof(TempHeader)), sums,
+                     norm, max_norm);
 }
