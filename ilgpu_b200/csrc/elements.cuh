@@ -89,6 +89,18 @@ template <typename T, int G> struct Group {
             *reinterpret_cast<unsigned short *>(p) = (unsigned short)w[0];
         }
     }
+    // For what is not read again soon.
+    __device__ __forceinline__ void store_streaming(T *p) const {
+        if constexpr (kBytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i)
+                __stcs(reinterpret_cast<uint4 *>(p) + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+        } else if constexpr (kBytes == 8) {
+            __stcs(reinterpret_cast<uint2 *>(p), make_uint2(w[0], w[1]));
+        } else {
+            store(p);
+        }
+    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0u;

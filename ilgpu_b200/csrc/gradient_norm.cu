@@ -20,16 +20,18 @@ constexpr int kMaxBlocks = 148 * kNormBlocksPerSm;  // partial sums of a launch
 constexpr int kMostViews = 1024;                    // of a launch: 30 KB of parameters
 constexpr int kMostSpan = 8;                        // chunks that a block takes one behind the other
 
-struct ViewTable {
-    const void *in[kMostViews];
-    void *out[kMostViews];
-    long long length[kMostViews];
-    unsigned int chunk[kMostViews + 1];  // first chunk of a view
-    unsigned char in_type[kMostViews], out_type[kMostViews];
+constexpr int kFewViews = 64;                       // of a launch with a short list: 2 KB of parameters cost the host 1 us less
+
+template <int MOST> struct ViewTable {
+    const void *in[MOST];
+    void *out[MOST];
+    long long length[MOST];
+    unsigned int chunk[MOST + 1];  // first chunk of a view
+    unsigned char in_type[MOST], out_type[MOST];
     int views;
     int span;
 };
-static_assert(sizeof(ViewTable) <= 31 << 10, "fits a kernel's parameters");
+static_assert(sizeof(ViewTable<kMostViews>) <= 31 << 10, "fits a kernel's parameters");
 
 // 16-byte groups of a view, from the boundary at or in front of its first element on.
 __host__ __device__ __forceinline__ int64_t groups_of(const void *p, int64_t length, int bytes) {
@@ -37,12 +39,13 @@ __host__ __device__ __forceinline__ int64_t groups_of(const void *p, int64_t len
 }
 
 // Views from `first` on that one launch takes; returns how many.
-static int64_t fill_table(ViewTable &t, const void *const *in, void *const *out, const int64_t *lengths, const int *in_types, const int *out_types,
+template <int MOST>
+static int64_t fill_table(ViewTable<MOST> &t, const void *const *in, void *const *out, const int64_t *lengths, const int *in_types, const int *out_types,
                           int64_t first, int64_t views) {
     int64_t i = first;
     unsigned int chunks = 0;
     t.views = 0;
-    for (; i < views && t.views < kMostViews; ++i) {
+    for (; i < views && t.views < MOST; ++i) {
         if (!lengths[i]) continue;
         const int v = t.views++;
         t.in[v] = in[i];
@@ -59,17 +62,26 @@ static int64_t fill_table(ViewTable &t, const void *const *in, void *const *out,
     return i - first;
 }
 
-// The chunks of a block: spans of a few one behind the other, taken in turn by all blocks, so that all of them read the
-// same part of memory at a time (a stretch of its own for each block: 5.4 TB/s instead of XX).  LAST_FIRST: from the end on.
-template <bool LAST_FIRST> struct Chunks {
-    const ViewTable &t;
-    unsigned int span, chunk, left;  // left: chunks of the span behind this one
+// The chunks of a block: spans of a few one behind the other, taken in turn by all blocks, so that all of
+// them read the same part of memory at a time (with a stretch of its own for each block 10^9 floats took 743 us instead of
+// 605).  LAST_FIRST: the same ones from the end on.
+template <bool LAST_FIRST, typename Table> struct Chunks {
+    const Table &t;
+    unsigned int chunk, left;  // left: chunks of the span that are still to come
     int view;
-    __device__ __forceinline__ Chunks(const ViewTable &table) : t(table), span(blockIdx.x) {}
-    __device__ __forceinline__ unsigned int spans() const { return (t.chunk[t.views] + t.span - 1) / t.span; }
+    int64_t span, step, spans;
+    __device__ __forceinline__ Chunks(const Table &table) : t(table) {
+        spans = (t.chunk[t.views] + t.span - 1) / t.span;
+        span = blockIdx.x;
+        step = gridDim.x;
+        if (LAST_FIRST) {
+            span = span < spans ? span + (spans - 1 - span) / step * step : -1;
+            step = -step;
+        }
+    }
     __device__ __forceinline__ bool enter() {
-        if (span >= spans()) return false;
-        const unsigned int at = LAST_FIRST ? spans() - 1 - span : span, begin = at * t.span, behind = begin + t.span;
+        if (span < 0 || span >= spans) return false;
+        const unsigned int begin = (unsigned int)span * t.span, behind = begin + t.span;
         const unsigned int end = behind < t.chunk[t.views] ? behind : t.chunk[t.views];
         left = end - begin - 1;
         chunk = LAST_FIRST ? end - 1 : begin;
@@ -84,7 +96,7 @@ template <bool LAST_FIRST> struct Chunks {
     }
     __device__ __forceinline__ bool next() {
         if (!left) {
-            span += gridDim.x;
+            span += step;
             return enter();
         }
         --left;
@@ -118,8 +130,9 @@ template <typename T> __device__ __forceinline__ uint4 edge_group(const T *in, i
     return make_uint4(g.w[0], g.w[1], g.w[2], g.w[3]);
 }
 
-// Loads this thread's part of the chunk; LAST: the data is not needed again.
-template <typename Where> __device__ __forceinline__ void load_part(Part &part, const ViewTable &t, const Where &at) {
+// Loads this thread's part of the chunk; KEEP: the data is wanted again.
+template <bool KEEP, typename Table, typename Where>
+__device__ __forceinline__ void load_part(Part &part, const Table &t, const Where &at) {
     const int v = at.view;
     part.view = v;
     part.type = t.in_type[v];
@@ -133,7 +146,7 @@ template <typename Where> __device__ __forceinline__ void load_part(Part &part, 
     for (int u = 0; u < kAheadGroups; ++u) {
         const int64_t g = part.group + u * kNormThreads;
         if (g < whole && (g || !before)) {
-            part.w[u] = __ldcs(reinterpret_cast<const uint4 *>(base) + g);
+            part.w[u] = KEEP ? reinterpret_cast<const uint4 *>(base)[g] : __ldcs(reinterpret_cast<const uint4 *>(base) + g);
         } else if (g * kGroupBytes < bytes) {
             const int64_t first = (g * kGroupBytes - before) >> shift;
             part.w[u] = shift == 2 ? edge_group((const float *)t.in[v], first, t.length[v]) : edge_group((const __half *)t.in[v], first, t.length[v]);
@@ -199,25 +212,30 @@ __device__ __forceinline__ float norm_of(const double *partial, int count) {
     return (float)sqrt(block_sum(sum));
 }
 
-__global__ void __launch_bounds__(kNormThreads) norm_partial_kernel(const __grid_constant__ ViewTable t, double *partial) {
-    grid_dependency_release();
-    Chunks<false> at(t);
+// The squares of the block's chunks, this thread's part of them.
+template <bool KEEP, typename Table> __device__ __forceinline__ double sum_squares(const Table &t) {
+    Chunks<false, Table> at(t);
     bool more = at.enter();
     grid_dependency_wait();
     double sum = 0.0;
     Part next;
-    if (more) load_part(next, t, at);
+    if (more) load_part<KEEP>(next, t, at);
     while (more) {  // the next chunk is under way while this one is added up
         const Part part = next;
         more = at.next();
-        if (more) load_part(next, t, at);
+        if (more) load_part<KEEP>(next, t, at);
         switch (part.type) {
         case B200ALG_F32: sum += squares<float>(part); break;
         case B200ALG_F16: sum += squares<__half>(part); break;
         default: sum += squares<__nv_bfloat16>(part);
         }
     }
-    sum = block_sum(sum);
+    return sum;
+}
+
+template <int MOST, bool KEEP> __global__ void __launch_bounds__(kNormThreads) norm_partial_kernel(const __grid_constant__ ViewTable<MOST> t, double *partial) {
+    grid_dependency_release();
+    const double sum = block_sum(sum_squares<KEEP>(t));
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
@@ -228,7 +246,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(const double 
     if (threadIdx.x == 0) *norm = whole;
 }
 
-template <typename TIn, typename TOut> __device__ __forceinline__ void scale_part(const Part &part, const ViewTable &t, float factor) {
+template <typename TIn, typename TOut, typename Table> __device__ __forceinline__ void scale_part(const Part &part, const Table &t, float factor) {
     constexpr int G = kGroupBytes / (int)sizeof(TIn);
     constexpr unsigned int kBoundary = G * sizeof(TOut) < 16 ? G * sizeof(TOut) : 16;
     const int64_t length = t.length[part.view];
@@ -246,7 +264,7 @@ template <typename TIn, typename TOut> __device__ __forceinline__ void scale_par
         if (first >= 0 && first + G <= length && (uintptr_t)to % kBoundary == 0) {
             Group<TOut, G> y;
             y.set(x);
-            y.store(to);
+            y.store_streaming(to);
         } else {
 #pragma unroll
             for (int k = 0; k < G; ++k)
@@ -255,7 +273,7 @@ template <typename TIn, typename TOut> __device__ __forceinline__ void scale_par
     }
 }
 
-template <typename TIn> __device__ __forceinline__ void scale_part_from(const Part &part, const ViewTable &t, float factor) {
+template <typename TIn, typename Table> __device__ __forceinline__ void scale_part_from(const Part &part, const Table &t, float factor) {
     switch (t.out_type[part.view]) {
     case B200ALG_F32: scale_part<TIn, float>(part, t, factor); break;
     case B200ALG_F16: scale_part<TIn, __half>(part, t, factor); break;
@@ -263,15 +281,22 @@ template <typename TIn> __device__ __forceinline__ void scale_part_from(const Pa
     }
 }
 
+// What the values are multiplied by.  A norm that is not finite leaves them as they are: it says so itself.
+__device__ __forceinline__ float factor_of(float norm, double max_norm) {
+    return norm <= FLT_MAX && (double)norm > max_norm ? (float)(max_norm / (double)norm) : 1.0f;
+}
+
+// Backwards, and each block what it has read for the norm: what was read last may still be in the cache.
 // partial == NULL: by the norm that is there; else the norm comes from the blocks' sums, and the first block stores it.
 // (Every block adds them up itself, so that no launch stands between the two passes.)
-__global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_constant__ ViewTable t, const double *partial, int count, float *norm, double max_norm) {
+template <int MOST>
+__global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_constant__ ViewTable<MOST> t, const double *partial, int count, float *norm, double max_norm) {
     grid_dependency_release();
-    Chunks<true> at(t);  // backwards: what the norm's pass has read last may still be in the cache
+    Chunks<true, ViewTable<MOST>> at(t);
     bool more = at.enter();
     grid_dependency_wait();
     Part next;
-    if (more) load_part(next, t, at);
+    if (more) load_part<false>(next, t, at);
     float whole;
     if (partial) {
         whole = norm_of(partial, count);
@@ -279,12 +304,11 @@ __global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_consta
     } else {
         whole = *norm;
     }
-    // a norm that is not finite leaves the values as they are: it says so itself
-    const float factor = whole <= FLT_MAX && (double)whole > max_norm ? (float)(max_norm / (double)whole) : 1.0f;
+    const float factor = factor_of(whole, max_norm);
     while (more) {
         const Part part = next;
         more = at.next();
-        if (more) load_part(next, t, at);
+        if (more) load_part<false>(next, t, at);
         if (factor == 1.0f && t.in[part.view] == t.out[part.view]) continue;
         switch (part.type) {
         case B200ALG_F32: scale_part_from<float>(part, t, factor); break;
@@ -294,7 +318,7 @@ __global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_consta
     }
 }
 
-static int blocks_of(const ViewTable &t) {
+template <int MOST> static int blocks_of(const ViewTable<MOST> &t) {
     const int64_t most = kMaxBlocks < (int64_t)sm_count() * kNormBlocksPerSm ? kMaxBlocks : (int64_t)sm_count() * kNormBlocksPerSm;
     const int64_t spans = ceil_div(t.chunk[t.views], t.span);
     return (int)(spans < most ? spans : most);
@@ -337,39 +361,52 @@ static int64_t norm_temp_bytes(int64_t count) {
     return sizeof(TempHeader) + round_up((ceil_div(count, kMostViews) + 1) * kMaxBlocks * 8, 256);  // every launch but the last takes kMostViews views
 }
 
+// A call's lists.
+struct ViewLists {
+    const void *const *in;
+    void *const *out;
+    const int64_t *lengths;
+    const int *in_types, *out_types;
+    int64_t count;
+};
+
 // The sums of squares of all launches' blocks; *sums: how many there are.
-static int run_partial(cudaStream_t s, const void *const *views, const int64_t *lengths, const int *types, int64_t count, void *temp, int *sums) {
-    double *partial = (double *)((char *)temp + sizeof(TempHeader));
+template <int MOST> static int run_partial(cudaStream_t s, const ViewLists &l, bool keep, double *partial, int *sums) {
     *sums = 0;
-    ViewTable t;
-    for (int64_t first = 0; first < count;) {
-        first += fill_table(t, views, nullptr, lengths, types, nullptr, first, count);
+    ViewTable<MOST> t;
+    for (int64_t first = 0; first < l.count;) {
+        first += fill_table(t, l.in, nullptr, l.lengths, l.in_types, nullptr, first, l.count);
         if (!t.views) break;
         const int blocks = blocks_of(t);
         double *to = partial + *sums;
         void *arguments[] = {&t, &to};
-        B200ALG_CUDA_TRY(launch_with_table((const void *)norm_partial_kernel, blocks, s, arguments));
+        B200ALG_CUDA_TRY(launch_with_table(keep ? (const void *)norm_partial_kernel<MOST, true> : (const void *)norm_partial_kernel<MOST, false>, blocks, s, arguments));
         *sums += blocks;
     }
     return B200ALG_OK;
 }
 
-static int run_finish(cudaStream_t s, int sums, float *norm, void *temp) {
-    B200ALG_CUDA_TRY(launch_dependent(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, (const double *)((char *)temp + sizeof(TempHeader)), sums, norm));
+// By the norm that is there (partial == NULL), or by that of `sums` partial sums, which the first launch stores.
+template <int MOST> static int run_scale(cudaStream_t s, const ViewLists &l, const double *partial, int sums, float *norm, double max_norm) {
+    ViewTable<MOST> t;
+    for (int64_t first = 0; first < l.count;) {
+        first += fill_table(t, l.in, l.out, l.lengths, l.in_types, l.out_types, first, l.count);
+        if (!t.views) break;
+        void *arguments[] = {&t, &partial, &sums, &norm, &max_norm};
+        B200ALG_CUDA_TRY(launch_with_table((const void *)scale_kernel<MOST>, blocks_of(t), s, arguments));
+        partial = nullptr;  // the norm is there now
+    }
     return B200ALG_OK;
 }
 
-// By the norm that is there (partial == NULL), or by that of `sums` partial sums, which the first launch stores.
-static int run_scale(cudaStream_t s, const void *const *views, void *const *outputs, const int64_t *lengths, const int *types, const int *out_types,
-                     int64_t count, const double *partial, int sums, float *norm, double max_norm) {
-    ViewTable t;
-    for (int64_t first = 0; first < count;) {
-        first += fill_table(t, views, outputs, lengths, types, out_types, first, count);
-        if (!t.views) break;
-        void *arguments[] = {&t, &partial, &sums, &norm, &max_norm};
-        B200ALG_CUDA_TRY(launch_with_table((const void *)scale_kernel, blocks_of(t), s, arguments));
-        partial = nullptr;  // the norm is there now
-    }
+// The norm, and with max_norm >= 0 the clipping by it.
+template <int MOST> static int run_clip(cudaStream_t s, const ViewLists &l, float *norm, double max_norm, void *temp) {
+    double *partial = (double *)((char *)temp + sizeof(TempHeader));
+    int sums = 0;
+    const int rc = run_partial<MOST>(s, l, max_norm >= 0.0, partial, &sums);
+    if (rc != B200ALG_OK) return rc;
+    if (max_norm >= 0.0) return run_scale<MOST>(s, l, partial, sums, norm, max_norm);
+    B200ALG_CUDA_TRY(launch_dependent(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, (const double *)partial, sums, norm));
     return B200ALG_OK;
 }
 
@@ -391,9 +428,9 @@ extern "C" int b200alg_gradient_norm(void *stream, const void *const *views, con
     if (!norm || !temp) return B200ALG_INVALID_ARGUMENT;
     if ((uintptr_t)norm % 4 || (uintptr_t)temp % 256) return B200ALG_MISALIGNED;
     if (temp_bytes < norm_temp_bytes(count)) return B200ALG_TEMP_TOO_SMALL;
-    int sums = 0;
-    const int status = run_partial((cudaStream_t)stream, views, lengths, dtypes, count, temp, &sums);
-    return status != B200ALG_OK ? status : run_finish((cudaStream_t)stream, sums, norm, temp);
+    const ViewLists l{views, nullptr, lengths, dtypes, nullptr, count};
+    if (count <= kFewViews) return run_clip<kFewViews>((cudaStream_t)stream, l, norm, -1.0, temp);
+    return run_clip<kMostViews>((cudaStream_t)stream, l, norm, -1.0, temp);
 }
 
 extern "C" int b200alg_gradient_scale(void *stream, const void *const *views, void *const *outputs, const int64_t *lengths, const int *dtypes,
@@ -402,20 +439,19 @@ extern "C" int b200alg_gradient_scale(void *stream, const void *const *views, vo
     if (rc != B200ALG_OK) return rc;
     if (!norm || !(max_norm >= 0.0)) return B200ALG_INVALID_ARGUMENT;
     if ((uintptr_t)norm % 4) return B200ALG_MISALIGNED;
-    return run_scale((cudaStream_t)stream, views, outputs, lengths, dtypes, out_dtypes, count, nullptr, 0, (float *)norm, max_norm);
+    const ViewLists l{views, outputs, lengths, dtypes, out_dtypes, count};
+    if (count <= kFewViews) return run_scale<kFewViews>((cudaStream_t)stream, l, nullptr, 0, (float *)norm, max_norm);
+    return run_scale<kMostViews>((cudaStream_t)stream, l, nullptr, 0, (float *)norm, max_norm);
 }
 
 extern "C" int b200alg_gradient_clip(void *stream, const void *const *views, void *const *outputs, const int64_t *lengths, const int *dtypes,
                                      const int *out_dtypes, int64_t count, double max_norm, float *norm, void *temp, int64_t temp_bytes) {
-    int rc = check_views(views, outputs, lengths, dtypes, out_dtypes, count);
+    const int rc = check_views(views, outputs, lengths, dtypes, out_dtypes, count);
     if (rc != B200ALG_OK) return rc;
     if (!norm || !temp || !(max_norm >= 0.0)) return B200ALG_INVALID_ARGUMENT;
     if ((uintptr_t)norm % 4 || (uintptr_t)temp % 256) return B200ALG_MISALIGNED;
     if (temp_bytes < norm_temp_bytes(count)) return B200ALG_TEMP_TOO_SMALL;
-    int sums = 0;
-    rc = run_partial((cudaStream_t)stream, views, lengths, dtypes, count, temp, &sums);
-    if (rc != B200ALG_OK) return rc;
-    if (!sums) return run_finish((cudaStream_t)stream, sums, norm, temp);  // nothing to clip
-    return run_scale((cudaStream_t)stream, views, outputs, lengths, dtypes, out_dtypes, count, (const double *)((char *)temp + sizeof(TempHeader)), sums,
-                     norm, max_norm);
+    const ViewLists l{views, outputs, lengths, dtypes, out_dtypes, count};
+    if (count <= kFewViews) return run_clip<kFewViews>((cudaStream_t)stream, l, norm, max_norm, temp);
+    return run_clip<kMostViews>((cudaStream_t)stream, l, norm, max_norm, temp);
 }
