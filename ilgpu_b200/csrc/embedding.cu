@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "elements.cuh"
+#include "sort_common.cuh"
 
 namespace b200alg {
 
@@ -69,13 +70,15 @@ static int run_lookup(cudaStream_t s, const void *table, int64_t rows, int64_t w
 // the other in the order of their positions; sums do not depend on how the work falls on the GPU.  A tile of sorted
 // positions is summed by the threads of a block, each holding one group of columns in registers and walking along the
 // tile.  A run of equal tokens inside a tile is written at once; a tile's share of a run that crosses its border goes to
-// temp, and gradient_join_kernel adds the shares up in order.  The same launch clears the rows that no token names.
+// temp, and gradient_join_kernel adds the shares up in order.  Rows that no token names, which are most of a large
+// table, are cleared by the other blocks of the same launch.  They know them from a bit per row and need not wait for the
+// sort, so that its time passes behind them.
 constexpr int kGradientThreads = 256;
-constexpr int kAhead = 8;      // rows a thread has in flight
-constexpr int kClearRows = 8;  // rows that a warp looks up and clears
+constexpr int kAhead = 8;      // rows, or shares, that a thread has in flight
 
 struct GradientCall {
     const unsigned int *keys, *positions;  // sorted
+    const unsigned int *named;             // a bit per row of the table
     int64_t n, tile, tiles;
     int64_t upstream_stride;
     int64_t rows, width, row_stride;
@@ -87,15 +90,26 @@ struct GradientCall {
     int x, y;           // threads of a block along the columns, tiles of a block
     int slabs;          // blocks along the columns
     int64_t sum_blocks;
+    int clear_rows;     // rows of a block that clears
+    int64_t clear_blocks;
+    int early;          // what clears need not wait for the launch before
 };
 
-static __global__ void __launch_bounds__(256) gradient_keys_kernel(IndexView tokens, int64_t n, int64_t rows, unsigned int *keys) {
+__global__ void __launch_bounds__(256) gradient_forget_kernel(uint4 *named, int64_t words) {
+    grid_dependency_release();
+    grid_dependency_wait();
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) named[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+__global__ void __launch_bounds__(256) gradient_keys_kernel(IndexView tokens, int64_t n, int64_t rows, unsigned int *keys, unsigned int *named) {
     grid_dependency_release();
     grid_dependency_wait();
     const int64_t step = (int64_t)gridDim.x * blockDim.x;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
         const int64_t token = tokens[i];
-        keys[i] = token >= 0 && token < rows ? (unsigned int)token : (unsigned int)rows;  // those without a row sort last
+        const bool there = token >= 0 && token < rows;
+        keys[i] = there ? (unsigned int)token : (unsigned int)rows;  // those without a row sort last
+        if (named && there) atomicOr(named + (token >> 5), 1u << (token & 31));
     }
 }
 
@@ -132,31 +146,38 @@ template <int G> __device__ __forceinline__ void write_share(float *p, const flo
     o.store(p);
 }
 
+// Clears those of the rows from `first` on, up to 32, whose bit in `rows` is set; by a warp.
+template <typename TOut, int G> __device__ __forceinline__ void clear_rows(const GradientCall &c, TOut *out, int64_t first, unsigned int rows) {
+    Group<TOut, G> zero;
+    zero.clear();
+    for (; rows; rows &= rows - 1) {
+        TOut *p = out + (first + __ffs(rows) - 1) * c.row_stride;
+        for (int g = threadIdx.x & 31; g < c.groups; g += 32) zero.store(p + (int64_t)g * G);
+    }
+}
+
 template <typename TIn, typename TOut, int G>
 __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(GradientCall c, const TIn *__restrict__ upstream, TOut *__restrict__ out) {
     grid_dependency_release();
-    grid_dependency_wait();
-    const unsigned int rows = (unsigned int)c.rows;
-    if (blockIdx.x >= c.sum_blocks) {  // rows that no token names
-        const int lane = threadIdx.x & 31;
-        const int64_t first = ((blockIdx.x - c.sum_blocks) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kClearRows;
-        bool empty = false;
-        if (lane < kClearRows && first + lane < c.rows) {
-            const unsigned int row = (unsigned int)(first + lane);
-            const int64_t at = lower_bound(c.keys, c.n, row);
-            empty = at == c.n || c.keys[at] != row;
-        }
-        Group<TOut, G> zero;
-        zero.clear();
-        for (unsigned int todo = __ballot_sync(0xffffffffu, empty); todo; todo &= todo - 1) {
-            TOut *p = out + (first + __ffs(todo) - 1) * c.row_stride;
-            for (int g = lane; g < c.groups; g += 32) zero.store(p + (int64_t)g * G);
+    if (blockIdx.x < c.clear_blocks) {
+        if (!c.early) grid_dependency_wait();
+        // a warp takes 32 rows, or where a block has fewer than that for each of them its part of them
+        const int warps = kGradientThreads / 32, each = c.clear_rows / warps < 1 ? 1 : c.clear_rows / warps;
+        const int64_t begin = (int64_t)blockIdx.x * c.clear_rows + (threadIdx.x >> 5) * each;
+        for (int64_t first = begin; first < begin + each && first < c.rows; first = (first | 31) + 1) {
+            const int from = (int)(first & 31);
+            const int64_t end = begin + each < c.rows ? begin + each : c.rows, most = (first | 31) + 1 < end ? 32 : (int)(end - (first - from));
+            unsigned int todo = ~c.named[first >> 5] & (~0u << from);
+            if (most < 32) todo &= (1u << most) - 1u;
+            clear_rows<TOut, G>(c, out, first - from, todo);
         }
         return;
     }
+    grid_dependency_wait();
+    const unsigned int rows = (unsigned int)c.rows, block = blockIdx.x - (unsigned int)c.clear_blocks;
     const int tx = threadIdx.x % c.x, ty = threadIdx.x / c.x;
-    const int64_t t = (int64_t)(blockIdx.x / c.slabs) * c.y + ty;
-    const int g = (int)(blockIdx.x % c.slabs) * c.x + tx;
+    const int64_t t = (int64_t)(block / c.slabs) * c.y + ty;
+    const int g = (int)(block % c.slabs) * c.x + tx;
     if (g >= c.groups || t >= c.tiles || ty >= c.y) return;
     const int64_t begin = t * c.tile, end = begin + c.tile < c.n ? begin + c.tile : c.n;
     const unsigned int *keys = c.keys;
@@ -214,17 +235,111 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
     if (c.keys[begin] == key && begin > 0 && c.keys[begin - 1] == key) return;           // it began in front of it
     const int64_t last = (lower_bound(c.keys + end, c.n - end, key + 1) + end - 1) / c.tile;  // the tile in which it ends
     float sum[G];
-    Group<float, G> share;
     const float *enters = c.shares + (int64_t)g * G;
-    share.load(enters + (c.tiles + t) * c.share_stride);
+    {
+        Group<float, G> share;
+        share.load(enters + (c.tiles + t) * c.share_stride);
 #pragma unroll
-    for (int k = 0; k < G; ++k) sum[k] = share.get(k);
-    for (int64_t i = t + 1; i <= last; ++i) {
-        share.load(enters + i * c.share_stride);
+        for (int k = 0; k < G; ++k) sum[k] = share.get(k);
+    }
+    for (int64_t i = t + 1; i <= last; i += kAhead) {
+        Group<float, G> share[kAhead];
 #pragma unroll
-        for (int k = 0; k < G; ++k) sum[k] += share.get(k);
+        for (int j = 0; j < kAhead; ++j) {
+            share[j].clear();
+            if (i + j <= last) share[j].load(enters + (i + j) * c.share_stride);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int k = 0; k < G; ++k) sum[k] += share[j].get(k);
     }
     write_row<TOut, G>(c, out, key, g, sum);
+}
+
+// ---- gradient of few tokens, in one launch ----
+// A block of a position looks all tokens over: if its token stands in front of it, another block has its row; else it
+// lists the positions that name the row and adds them up, in y parts that are joined in order.  What clears does so with
+// the bits of its own rows, from all tokens as well.  (Sorting them would take one block 13 us and the launches around it
+// 5, whatever the table.)
+constexpr int64_t kFewTokens = 1024;
+constexpr int kFewParts = 4;
+
+template <typename TIn, typename TOut, int G>
+__global__ void __launch_bounds__(kGradientThreads)
+gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ upstream, TOut *__restrict__ out, TempHeader *hdr) {
+    grid_dependency_release();
+    __shared__ unsigned int bits[kFewTokens / 32];
+    __shared__ unsigned short list[kFewTokens];
+    __shared__ float part[kGradientThreads * G];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (int)c.n;
+    if (blockIdx.x >= c.sum_blocks) {
+        const int64_t first = (blockIdx.x - c.sum_blocks) * c.clear_rows;  // clear_rows: 32 for each warp at most
+        if (threadIdx.x < kGradientThreads / 32) bits[threadIdx.x] = 0u;
+        __syncthreads();
+        grid_dependency_wait();
+        if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) hdr->wait_limit_hit = 0u;  // no wait can run out
+        for (int i = threadIdx.x; i < n; i += kGradientThreads) {
+            const int64_t at = tokens[i] - first;
+            if (at >= 0 && at < c.clear_rows) atomicOr(bits + (at >> 5), 1u << (at & 31));
+        }
+        __syncthreads();
+        for (int i = warp; i < c.clear_rows; i += kGradientThreads / 32)
+            if (first + i < c.rows && !(bits[i >> 5] >> (i & 31) & 1)) clear_rows<TOut, G>(c, out, first + i, 1u);
+        return;
+    }
+    grid_dependency_wait();
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) hdr->wait_limit_hit = 0u;
+    const int i = (int)(blockIdx.x / c.slabs);
+    const int64_t token = tokens[i];
+    if (token < 0 || token >= c.rows) return;
+    for (int base = 0; base < n; base += kGradientThreads) {
+        const int j = base + (int)threadIdx.x;
+        const unsigned int same = __ballot_sync(0xffffffffu, j < n && tokens[j] == token);
+        if (lane == 0 && base + warp * 32 < kFewTokens) bits[base / 32 + warp] = same;
+    }
+    __syncthreads();
+    const int words = (n + 31) / 32;
+    int count = 0;
+    bool earlier = false;
+    for (int w = 0; w < words; ++w) {  // (all threads alike)
+        const unsigned int same = bits[w];
+        if (w < i / 32 ? same : w == i / 32 && same << (31 - i % 32) << 1) earlier = true;
+        if (w % (kGradientThreads / 32) == warp && same >> lane & 1) list[count + __popc(same & lanemask_lt())] = (unsigned short)(w * 32 + lane);
+        count += __popc(same);
+    }
+    if (earlier) return;
+    __syncthreads();
+    const int x = kGradientThreads / kFewParts, tx = threadIdx.x % x, ty = threadIdx.x / x;
+    const int g = (int)(blockIdx.x % c.slabs) * x + tx;
+    const int begin = count * ty / kFewParts, end = count * (ty + 1) / kFewParts;
+    float sum[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) sum[k] = 0.0f;
+    for (int r = begin; r < end && g < c.groups; r += kAhead) {
+        Group<TIn, G> in[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            in[j].clear();
+            if (r + j < end) in[j].load(upstream + list[r + j] * c.upstream_stride + (int64_t)g * G);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int k = 0; k < G; ++k) sum[k] += in[j].get(k);
+    }
+#pragma unroll
+    for (int k = 0; k < G; ++k) part[k * kGradientThreads + threadIdx.x] = sum[k];
+    __syncthreads();
+    if (ty == 0 && g < c.groups) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+            sum[k] = part[k * kGradientThreads + tx];
+#pragma unroll
+            for (int p = 1; p < kFewParts; ++p) sum[k] += part[k * kGradientThreads + p * x + tx];
+        }
+        write_row<TOut, G>(c, out, (unsigned int)token, g, sum);
+    }
 }
 
 // Sorted positions of a tile: enough tiles for the GPU, and shares of crossing runs that stay a small part of the traffic.
@@ -236,7 +351,7 @@ static int64_t gradient_tile(int64_t n) {
 
 struct GradientLayout {
     int64_t tile, tiles, share_stride;
-    int64_t sort_bytes, off_keys, off_positions, off_shares, total;
+    int64_t sort_bytes, off_keys, off_positions, off_named, named_words, off_shares, total;
 };
 static int gradient_layout(int64_t rows, int64_t width, int64_t n, GradientLayout &L) {
     if (rows < 0 || width < 0 || n < 0) return B200ALG_INVALID_ARGUMENT;
@@ -248,25 +363,58 @@ static int gradient_layout(int64_t rows, int64_t width, int64_t n, GradientLayou
     if (rc != B200ALG_OK) return rc;
     L.off_keys = round_up(L.sort_bytes, 256);
     L.off_positions = L.off_keys + round_up(n * 4, 256);
-    L.off_shares = L.off_positions + round_up(n * 4, 256);
+    L.off_named = L.off_positions + round_up(n * 4, 256);
+    L.named_words = ceil_div(rows, 128);  // of 16 bytes
+    L.off_shares = L.off_named + round_up(L.named_words * 16, 256);
     L.total = L.off_shares + round_up(2 * L.tiles * L.share_stride * 4, 256);
     return B200ALG_OK;
 }
 
+// Rows that a block clears: about 64 KB of them.
+static int rows_to_clear(int64_t width, int bytes, int most) {
+    const int64_t rows = (64 << 10) / (width * bytes);
+    return (int)(rows < kGradientThreads / 32 ? kGradientThreads / 32 : rows > most ? most : rows / (kGradientThreads / 32) * (kGradientThreads / 32));
+}
+
 template <typename TIn, typename TOut, int G>
-static int run_gradient(cudaStream_t s, GradientCall c, const void *upstream, void *out) {
+static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens, const GradientLayout &L, const void *upstream, void *out, void *temp) {
     c.groups = (int)(c.width / G);
-    for (c.x = 32; c.x < kGradientThreads && c.x < c.groups; c.x *= 2) {}
+    char *t = (char *)temp;
+    if (c.n <= kFewTokens) {
+        c.slabs = (int)ceil_div(c.groups, kGradientThreads / kFewParts);
+        c.sum_blocks = c.n * c.slabs;
+        c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 256);
+        const int64_t blocks = c.sum_blocks + (c.accumulate ? 0 : ceil_div(c.rows, c.clear_rows));
+        if (blocks > INT32_MAX) return B200ALG_TOO_LARGE;
+        if (blocks)
+            B200ALG_CUDA_TRY(launch_dependent(gradient_few_kernel<TIn, TOut, G>, dim3((unsigned)blocks), dim3(kGradientThreads), 0, s, c, tokens,
+                                              (const TIn *)upstream, (TOut *)out, (TempHeader *)temp));
+        return B200ALG_OK;
+    }
+    unsigned int *keys = (unsigned int *)(t + L.off_keys), *positions = (unsigned int *)(t + L.off_positions);
+    unsigned int *named = c.accumulate ? nullptr : (unsigned int *)(t + L.off_named);
+    const int64_t cap = (int64_t)sm_count() * 8;
+    auto some = [&](int64_t want) { return dim3((unsigned)(want < cap ? want : cap)); };
+    if (named)
+        B200ALG_CUDA_TRY(launch_dependent(gradient_forget_kernel, some(ceil_div(L.named_words, 256)), dim3(256), 0, s, (uint4 *)named, L.named_words));
+    B200ALG_CUDA_TRY(launch_dependent(gradient_keys_kernel, some(ceil_div(c.n, 256 * 2)), dim3(256), 0, s, tokens, c.n, c.rows, keys, named));
+    bool one_launch = false;
+    const int rc = sort_with_positions(s, keys, positions, c.n, temp, L.sort_bytes, &one_launch);
+    if (rc != B200ALG_OK) return rc;
+    c.keys = keys, c.positions = positions, c.named = named;
+    c.tile = L.tile, c.tiles = L.tiles;
+    c.shares = (float *)(t + L.off_shares), c.share_stride = L.share_stride;
+    for (c.x = 8; c.x < kGradientThreads && c.x < c.groups; c.x *= 2) {}
     c.y = kGradientThreads / c.x;
     c.slabs = (int)ceil_div(c.groups, c.x);
     c.sum_blocks = ceil_div(c.tiles, c.y) * c.slabs;
-    const int64_t clear_blocks = c.accumulate ? 0 : ceil_div(c.rows, kClearRows * (kGradientThreads / 32));
-    if (c.sum_blocks + clear_blocks > INT32_MAX) return B200ALG_TOO_LARGE;
-    if (c.sum_blocks + clear_blocks > 0)
-        B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G>, dim3((unsigned)(c.sum_blocks + clear_blocks)), dim3(kGradientThreads), 0, s,
-                                          c, (const TIn *)upstream, (TOut *)out));
-    if (c.tiles > 1)
-        B200ALG_CUDA_TRY(launch_dependent(gradient_join_kernel<TOut, G>, dim3((unsigned)c.sum_blocks), dim3(kGradientThreads), 0, s, c, (TOut *)out));
+    c.early = one_launch;
+    c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 1 << 20);
+    c.clear_blocks = named ? ceil_div(c.rows, c.clear_rows) : 0;
+    if (c.sum_blocks + c.clear_blocks > INT32_MAX) return B200ALG_TOO_LARGE;
+    B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G>, dim3((unsigned)(c.sum_blocks + c.clear_blocks)), dim3(kGradientThreads), 0, s, c,
+                                      (const TIn *)upstream, (TOut *)out));
+    B200ALG_CUDA_TRY(launch_dependent(gradient_join_kernel<TOut, G>, dim3((unsigned)c.sum_blocks), dim3(kGradientThreads), 0, s, c, (TOut *)out));
     return B200ALG_OK;
 }
 
@@ -325,30 +473,20 @@ extern "C" int b200alg_embedding_gradient(void *stream, const void *tokens, int6
         return B200ALG_MISALIGNED;
     if (temp_bytes < L.total) return B200ALG_TEMP_TOO_SMALL;
     cudaStream_t s = (cudaStream_t)stream;
-    char *t = (char *)temp;
-    unsigned int *keys = (unsigned int *)(t + L.off_keys), *positions = (unsigned int *)(t + L.off_positions);
-    if (n) {
-        const IndexView view{tokens, token_stride, token_dtype == B200ALG_I64};
-        const int64_t want = ceil_div(n, 256 * 2), cap = (int64_t)sm_count() * 8;
-        B200ALG_CUDA_TRY(launch_dependent(gradient_keys_kernel, dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, s, view, n, rows, keys));
-        rc = b200alg_radix_sort_pairs_sequence(stream, keys, positions, n, B200ALG_U32, B200ALG_U32, B200ALG_SORT_ASCENDING, temp, L.sort_bytes);
-        if (rc != B200ALG_OK) return rc;
-    }
+    const IndexView view{tokens, token_stride, token_dtype == B200ALG_I64};
     GradientCall c{};
-    c.keys = keys, c.positions = positions;
-    c.n = n, c.tile = L.tile, c.tiles = L.tiles;
+    c.n = n;
     c.upstream_stride = upstream_stride;
     c.rows = rows, c.width = width, c.row_stride = row_stride;
     c.scale = (float)scale, c.accumulate = accumulate != 0;
-    c.shares = (float *)(t + L.off_shares), c.share_stride = L.share_stride;
     return with_element(upstream_dtype, [&](auto in) {
         return with_element(dtype, [&](auto to) {
             using TIn = decltype(in);
             using TOut = decltype(to);
             constexpr int G = 16 / sizeof(TIn);
             if (groups_aligned(upstream, upstream_stride, n, width, ib, G) && groups_aligned(gradient, row_stride, rows, width, ob, G))
-                return run_gradient<TIn, TOut, G>(s, c, upstream, gradient);
-            return run_gradient<TIn, TOut, 1>(s, c, upstream, gradient);
+                return run_gradient<TIn, TOut, G>(s, c, view, L, upstream, gradient, temp);
+            return run_gradient<TIn, TOut, 1>(s, c, view, L, upstream, gradient, temp);
         });
     });
 }

@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(const double 
 
 template <typename TIn, typename TOut, typename Table> __device__ __forceinline__ void scale_part(const Part &part, const Table &t, float factor) {
     constexpr int G = kGroupBytes / (int)sizeof(TIn);
-    constexpr unsigned int kBoundary = G * sizeof(TOut) < 16 ? G * sizeof(TOut) : 16;
+    constexpr unsigned int kBoundary = G * sizeof(TOut);
     const int64_t length = t.length[part.view];
     const int before = (int)((uintptr_t)t.in[part.view] & (kGroupBytes - 1)) / (int)sizeof(TIn);
 #pragma unroll

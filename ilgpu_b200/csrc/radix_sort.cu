@@ -1344,8 +1344,10 @@ static int partition_key(cudaStream_t s, int kb, const void *keys, const void *v
     return B200ALG_UNSUPPORTED;
 }
 
+// *one_launch: whether the sort was one launch.
 static int sort_common(void *stream, const SortCall &call, int key_dtype, int value_bytes, int order, void *temp,
-                       int64_t temp_bytes) {
+                       int64_t temp_bytes, bool *one_launch = nullptr) {
+    if (one_launch) *one_launch = false;
     // Argument checks mirror VerifyArguments (RadixSortExtensions.cs:1340-1367).
     if (!call.in_keys || !call.out_keys || !temp || (value_bytes && !call.out_values)) return B200ALG_INVALID_ARGUMENT;
     if (value_bytes && !call.in_values && call.value_seq == kSeqNone) return B200ALG_INVALID_ARGUMENT;
@@ -1370,10 +1372,13 @@ static int sort_common(void *stream, const SortCall &call, int key_dtype, int va
         bool taken = false;
         const SortScratch scratch{(char *)temp + L.off_keys, (char *)temp + L.off_values, L.control_bytes};
         int rc = block_sort(s, call, kb, value_bytes, xn, xp, temp, &taken);
+        if (one_launch) *one_launch = taken;
         if (rc != B200ALG_OK || taken) return rc;
         rc = sample_sort(s, call, kb, value_bytes, xn, xp, temp, scratch, &taken);
+        if (one_launch) *one_launch = taken;
         if (rc != B200ALG_OK || taken) return rc;
         rc = resident_sort(s, call, kb, value_bytes, xn, xp, temp, temp_bytes, &taken);
+        if (one_launch) *one_launch = taken;
         if (rc != B200ALG_OK || taken) return rc;
     }
     switch (value_bytes) {
@@ -1385,6 +1390,11 @@ static int sort_common(void *stream, const SortCall &call, int key_dtype, int va
     case 16: return dispatch_key<uint4>(s, kb, call, xn, xp, temp, L);
     }
     return B200ALG_UNSUPPORTED;
+}
+
+int sort_with_positions(void *stream, unsigned int *keys, unsigned int *positions, int64_t n, void *temp, int64_t temp_bytes, bool *one_launch) {
+    const SortCall call{keys, keys, positions, positions, 1, n, nullptr, kSeqInteger, false};
+    return sort_common(stream, call, B200ALG_U32, 4, B200ALG_SORT_ASCENDING, temp, temp_bytes, one_launch);
 }
 
 }  // namespace b200alg
