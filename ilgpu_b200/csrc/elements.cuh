@@ -65,7 +65,7 @@ template <typename T, int G> struct Group {
         static_assert(kBytes <= 32, "one instruction");
         if constexpr (kBytes == 32) {
             asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
         } else if constexpr (kBytes == 16) {
             const uint4 v = *reinterpret_cast<const uint4 *>(p);
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
