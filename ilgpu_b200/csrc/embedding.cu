@@ -383,7 +383,7 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
 // traffic.
 static int64_t gradient_tile(int64_t n) {
     int64_t tile = 128;
-    while (tile > 16 && ceil_div(n, tile) < 148 * 4) tile /= 2;
+    while (tile > 16 && ceil_div(n, tile) < 148 * 3 / 2) tile /= 2;
     return tile;
 }
 
