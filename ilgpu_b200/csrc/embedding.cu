@@ -11,57 +11,131 @@
 
 namespace b200alg {
 
+// Where rows do not lie on boundaries that groups can be moved from and to whole, groups of four columns begin on the
+// boundaries of the OUTPUT row (the first and the last one of a row stick out of it), and are put together from the two
+// aligned words of the input that hold them.  SHIFTED below.  (One element at a time instead: XX.)
+constexpr int kShiftedGroup = 4;
+
+// Extent of a matrix that is read: a word that overlaps it may be loaded whole (an aligned word lies in one page).
+struct Extent {
+    const char *begin, *end;
+};
+inline Extent extent_of(const void *p, int64_t rows, int64_t width, int64_t row_stride, int bytes) {
+    return Extent{(const char *)p, (const char *)p + (rows ? (rows - 1) * row_stride + width : 0) * bytes};
+}
+
+template <typename T, int G, bool SHIFTED> struct Columns {  // G columns of a row, as they are loaded
+    Group<T, G> w;
+    __device__ __forceinline__ void load(const T *p, const Extent &) { w.load(p); }
+    __device__ __forceinline__ void clear() { w.clear(); }
+    __device__ __forceinline__ Group<T, G> get() const { return w; }
+};
+template <typename T, int G> struct Columns<T, G, true> {
+    static_assert(G == kShiftedGroup, "two words, of which four elements are chosen");
+    Group<T, G> w, behind;
+    int shift;  // elements of w in front of the first column
+    __device__ __forceinline__ void load(const T *p, const Extent &matrix) {
+        constexpr int kBytes = Group<T, G>::kBytes;
+        const char *word = (const char *)((uintptr_t)p & ~(uintptr_t)(kBytes - 1));
+        shift = (int)(((const char *)p - word) / (int)sizeof(T));
+        if (word + kBytes > matrix.begin && word < matrix.end) w.load((const T *)word);
+        else w.clear();
+        if (shift && word + kBytes < matrix.end) behind.load((const T *)(word + kBytes));
+        else behind.clear();
+    }
+    __device__ __forceinline__ void clear() {
+        w.clear();
+        behind.clear();
+        shift = 0;
+    }
+    __device__ __forceinline__ Group<T, G> get() const {
+        Group<T, G> r;
+        if constexpr (sizeof(T) == 4) {
+            unsigned int t[5];
+            const unsigned int all[8] = {w.w[0], w.w[1], w.w[2], w.w[3], behind.w[0], behind.w[1], behind.w[2], behind.w[3]};
+#pragma unroll
+            for (int i = 0; i < 5; ++i) t[i] = shift & 2 ? all[i + 2] : all[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.w[i] = shift & 1 ? t[i + 1] : t[i];
+        } else {
+            const unsigned int a = shift & 2 ? w.w[1] : w.w[0], b = shift & 2 ? behind.w[0] : w.w[1], c = shift & 2 ? behind.w[1] : behind.w[0];
+            r.w[0] = __funnelshift_r(a, b, shift % 2 * 16);
+            r.w[1] = __funnelshift_r(b, c, shift % 2 * 16);
+        }
+        return r;
+    }
+};
+
+// First column of a group of the output row.
+template <bool SHIFTED, int G, typename T> __device__ __forceinline__ int64_t column_of(const T *row, int64_t g) {
+    return SHIFTED ? g * G - (int64_t)((uintptr_t)row / sizeof(T) % G) : g * G;
+}
+// Writes y to the columns from `column` on that the row has.
+template <bool SHIFTED, typename T, int G> __device__ __forceinline__ void put_columns(T *row, int64_t column, int64_t width, const float (&y)[G]) {
+    if (!SHIFTED || (column >= 0 && column + G <= width)) {
+        Group<T, G> o;
+        o.set(y);
+        o.store(row + column);
+    } else {
+#pragma unroll
+        for (int k = 0; k < G; ++k)
+            if (column + k >= 0 && column + k < width) row[column + k] = from_float<T>(y[k]);
+    }
+}
+// Groups of a row.
+inline int64_t groups_in(int64_t width, int group, bool shifted) { return shifted ? (width + 2 * group - 2) / group : width / group; }
+
 // ---- lookup --------------------------------------------------------------------------------
 // Nothing but memory traffic: a thread moves kLookupItems groups of up to 32 bytes, loads ahead of stores.  A group's row
 // and column come from one division by the groups of a row, so that rows of any width fill the warps.  (65536 rows of
 // 4096 bf16 out of 128000: groups of 16 bytes 127 us, of 32 bytes 114.6, four of those 116.)
 constexpr int kLookupThreads = 256, kLookupItems = 2;
 
-template <typename TIn, typename TOut, int G>
+template <typename TIn, typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kLookupThreads)
-lookup_kernel(const TIn *__restrict__ table, int64_t rows, int64_t row_stride, IndexView tokens, int64_t first, TOut *__restrict__ out,
-              int64_t out_stride, unsigned int total, FastDivide groups, float scale) {
+lookup_kernel(const TIn *__restrict__ table, int64_t rows, int64_t width, int64_t row_stride, Extent extent, IndexView tokens, int64_t first,
+              TOut *__restrict__ out, int64_t out_stride, unsigned int total, FastDivide groups, float scale) {
     grid_dependency_release();
     grid_dependency_wait();
     const unsigned int base = blockIdx.x * (kLookupThreads * kLookupItems) + threadIdx.x;
-    Group<TIn, G> in[kLookupItems];
+    Columns<TIn, G, SHIFTED> in[kLookupItems];
     TOut *to[kLookupItems];
+    int64_t column[kLookupItems];
 #pragma unroll
     for (int u = 0; u < kLookupItems; ++u) {
         const unsigned int q = base + u * kLookupThreads;
         to[u] = nullptr;
         if (q < total) {
             const unsigned int row = groups(q);
-            const int64_t column = (int64_t)(q - row * groups.d) * G;
             const int64_t token = tokens[first + row];
-            to[u] = out + (first + row) * out_stride + column;
-            if (token >= 0 && token < rows) in[u].load(table + token * row_stride + column);
+            to[u] = out + (first + row) * out_stride;
+            column[u] = column_of<SHIFTED, G>(to[u], q - row * groups.d);
+            if (token >= 0 && token < rows) in[u].load(table + token * row_stride + column[u], extent);
             else in[u].clear();
         }
     }
 #pragma unroll
     for (int u = 0; u < kLookupItems; ++u) {
         if (!to[u]) continue;
+        const Group<TIn, G> g = in[u].get();
         float x[G];
 #pragma unroll
-        for (int k = 0; k < G; ++k) x[k] = in[u].get(k) * scale;
-        Group<TOut, G> y;
-        y.set(x);
-        y.store(to[u]);
+        for (int k = 0; k < G; ++k) x[k] = g.get(k) * scale;
+        put_columns<SHIFTED>(to[u], column[u], width, x);
     }
 }
 
-template <typename TIn, typename TOut, int G>
+template <typename TIn, typename TOut, int G, bool SHIFTED>
 static int run_lookup(cudaStream_t s, const void *table, int64_t rows, int64_t width, int64_t row_stride, const IndexView &tokens, int64_t n,
                       double scale, void *out, int64_t out_stride) {
-    const int64_t groups = width / G;
+    const int64_t groups = groups_in(width, G, SHIFTED);
     const int64_t most = (((int64_t)1 << 31) - kLookupThreads * kLookupItems) / groups;  // rows of a launch, whose groups 31 bits count
     if (most < 1) return B200ALG_TOO_LARGE;
     for (int64_t first = 0; first < n; first += most) {
         const int64_t total = (n - first < most ? n - first : most) * groups;
-        B200ALG_CUDA_TRY(launch_dependent(lookup_kernel<TIn, TOut, G>, dim3((unsigned)ceil_div(total, kLookupThreads * kLookupItems)),
-                                          dim3(kLookupThreads), 0, s, (const TIn *)table, rows, row_stride, tokens, first, (TOut *)out, out_stride,
-                                          (unsigned int)total, FastDivide((unsigned int)groups), (float)scale));
+        B200ALG_CUDA_TRY(launch_dependent(lookup_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)ceil_div(total, kLookupThreads * kLookupItems)),
+                                          dim3(kLookupThreads), 0, s, (const TIn *)table, rows, width, row_stride,
+                                          extent_of(table, rows, width, row_stride, sizeof(TIn)), tokens, first, (TOut *)out, out_stride, (unsigned int)total, FastDivide((unsigned int)groups), (float)scale));
     }
     return B200ALG_OK;
 }
@@ -82,6 +156,7 @@ struct GradientCall {
     const unsigned char *named;            // a byte per row of the table: whether a token names it
     int64_t n, tile, tiles;
     int64_t upstream_stride;
+    Extent extent;      // of upstream
     int64_t rows, width, row_stride;
     float scale;
     int accumulate;
@@ -116,21 +191,25 @@ __global__ void __launch_bounds__(256) gradient_keys_kernel(IndexView tokens, in
     }
 }
 
-template <typename TOut, int G>
+// The scaled sum to group g of a row of the table's gradient.
+template <bool SHIFTED, typename TOut, int G>
 __device__ __forceinline__ void write_row(const GradientCall &c, TOut *out, unsigned int key, int g, const float (&sum)[G]) {
-    TOut *p = out + (int64_t)key * c.row_stride + (int64_t)g * G;
+    TOut *row = out + (int64_t)key * c.row_stride;
+    const int64_t column = column_of<SHIFTED, G>(row, g);
     float y[G];
-    Group<TOut, G> o;
-    if (c.accumulate) {
-        o.load(p);
+    if (!c.accumulate) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) y[k] = sum[k] * c.scale;
+    } else if (!SHIFTED || (column >= 0 && column + G <= c.width)) {
+        Group<TOut, G> o;
+        o.load(row + column);
 #pragma unroll
         for (int k = 0; k < G; ++k) y[k] = fmaf(sum[k], c.scale, o.get(k));
     } else {
 #pragma unroll
-        for (int k = 0; k < G; ++k) y[k] = sum[k] * c.scale;
+        for (int k = 0; k < G; ++k) y[k] = column + k >= 0 && column + k < c.width ? fmaf(sum[k], c.scale, to_float(row[column + k])) : 0.0f;
     }
-    o.set(y);
-    o.store(p);
+    put_columns<SHIFTED>(row, column, c.width, y);
 }
 template <int G> __device__ __forceinline__ void write_share(float *p, const float (&sum)[G]) {
     Group<float, G> o;
@@ -139,16 +218,17 @@ template <int G> __device__ __forceinline__ void write_share(float *p, const flo
 }
 
 // Clears those of the rows from `first` on, up to 32, whose bit in `rows` is set; by a warp.
-template <typename TOut, int G> __device__ __forceinline__ void clear_rows(const GradientCall &c, TOut *out, int64_t first, unsigned int rows) {
-    Group<TOut, G> zero;
-    zero.clear();
+template <bool SHIFTED, int G, typename TOut> __device__ __forceinline__ void clear_rows(const GradientCall &c, TOut *out, int64_t first, unsigned int rows) {
+    float zero[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) zero[k] = 0.0f;
     for (; rows; rows &= rows - 1) {
-        TOut *p = out + (first + __ffs(rows) - 1) * c.row_stride;
-        for (int g = threadIdx.x & 31; g < c.groups; g += 32) zero.store(p + (int64_t)g * G);
+        TOut *row = out + (first + __ffs(rows) - 1) * c.row_stride;
+        for (int g = threadIdx.x & 31; g < c.groups; g += 32) put_columns<SHIFTED>(row, column_of<SHIFTED, G>(row, g), c.width, zero);
     }
 }
 
-template <typename TIn, typename TOut, int G>
+template <typename TIn, typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(GradientCall c, const TIn *__restrict__ upstream, TOut *__restrict__ out) {
     grid_dependency_release();
     if (blockIdx.x < c.clear_blocks) {
@@ -156,7 +236,7 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(Gradient
         const int lane = threadIdx.x & 31, each = c.clear_rows / (kGradientThreads / 32);  // rows of a warp
         const int64_t begin = (int64_t)blockIdx.x * c.clear_rows + (threadIdx.x >> 5) * each, end = begin + each < c.rows ? begin + each : c.rows;
         for (int64_t first = begin; first < end; first += 32)
-            clear_rows<TOut, G>(c, out, first, __ballot_sync(0xffffffffu, first + lane < end && !c.named[first + lane]));
+            clear_rows<SHIFTED, G>(c, out, first, __ballot_sync(0xffffffffu, first + lane < end && !c.named[first + lane]));
         return;
     }
     grid_dependency_wait();
@@ -185,11 +265,13 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(Gradient
     __syncthreads();
     const int len = length;
     if (g >= c.groups || !len) return;
-    const TIn *const from = upstream + (int64_t)g * G;
-    Group<TIn, G> in[kAhead];  // a row is replaced by the one kAhead behind it as soon as it has been added
+    auto fetch = [&](Columns<TIn, G, SHIFTED> &to, int i) {  // what the i-th position of the tile has in the columns of its row
+        to.load(upstream + (int64_t)position[i] * c.upstream_stride + column_of<SHIFTED, G>(out + (int64_t)key[i] * c.row_stride, g), c.extent);
+    };
+    Columns<TIn, G, SHIFTED> in[kAhead];  // a row is replaced by the one kAhead behind it as soon as it has been added
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-        if (j < len) in[j].load(from + (int64_t)position[j] * c.upstream_stride);
+        if (j < len) fetch(in[j], j);
     unsigned int current = key[0];
     bool entered = key[-1] == current;  // whether the current run began in front of the tile
     float sum[G];
@@ -203,37 +285,43 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(Gradient
             const unsigned int next = key[i + j];
             if (next != current) {
                 if (entered) write_share<G>(enters, sum);
-                else write_row<TOut, G>(c, out, current, g, sum);
+                else write_row<SHIFTED>(c, out, current, g, sum);
                 entered = false;
                 current = next;
 #pragma unroll
                 for (int k = 0; k < G; ++k) sum[k] = 0.0f;
             }
+            const Group<TIn, G> x = in[j].get();
 #pragma unroll
-            for (int k = 0; k < G; ++k) sum[k] += in[j].get(k);
-            if (i + j + kAhead < len) in[j].load(from + (int64_t)position[i + j + kAhead] * c.upstream_stride);
+            for (int k = 0; k < G; ++k) sum[k] += x.get(k);
+            if (i + j + kAhead < len) fetch(in[j], i + j + kAhead);
         }
     }
     if (entered) write_share<G>(enters, sum);
     else if (len == tile && key[tile] == current) write_share<G>(leaves, sum);
-    else write_row<TOut, G>(c, out, current, g, sum);
+    else write_row<SHIFTED>(c, out, current, g, sum);
 }
 
-// Runs over several tiles: where one begins, its shares are added up.  The four parts of a block take a tile each; a run of
-// many shares is added up by all of them, and their sums are joined in order.
-constexpr int kParts = 4, kPartThreads = kGradientThreads / kParts;
+// Runs over several tiles: where one begins, its shares are added up.  A block is made of parts, each wide enough for its
+// columns.  They take a tile each; a run of many shares is added up by all of them, and their sums are joined in order.
+constexpr int kPartThreads = 64, kLeastPart = 8;  // threads of a part
+constexpr int kParts = kGradientThreads / kPartThreads, kMostParts = kGradientThreads / kLeastPart;
+static int part_threads(int groups) {
+    int x = kLeastPart;
+    while (x < kPartThreads && x < groups) x *= 2;
+    return x;
+}
 
-// Adds the parts' sums up, in those of the first one.
-template <int G> __device__ __forceinline__ void join_parts(float (&sum)[G], float *part, int tx, int ty) {
+// Adds the sums of the parts, of x threads each, up, in those of the first one.
+template <int G> __device__ __forceinline__ void join_parts(float (&sum)[G], float *part, int x) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < G; ++k) part[k * kGradientThreads + threadIdx.x] = sum[k];
     __syncthreads();
-    if (ty) return;
+    if (threadIdx.x >= x) return;
+    for (int p = x; p < kGradientThreads; p += x)
 #pragma unroll
-    for (int k = 0; k < G; ++k)
-#pragma unroll
-        for (int p = 1; p < kParts; ++p) sum[k] += part[k * kGradientThreads + p * kPartThreads + tx];
+        for (int k = 0; k < G; ++k) sum[k] += part[k * kGradientThreads + p + threadIdx.x];
 }
 
 // Adds the shares of the tiles [from, to) up: of the tile `start` what leaves it, of the others what enters them.
@@ -254,16 +342,16 @@ __device__ __forceinline__ void add_shares(float (&sum)[G], const GradientCall &
     }
 }
 
-template <typename TOut, int G>
-__global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(GradientCall c, TOut *__restrict__ out) {
+template <typename TOut, int G, bool SHIFTED>
+__global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(GradientCall c, TOut *__restrict__ out, int x) {
     __shared__ float part[kGradientThreads * G];
-    __shared__ int64_t ends[kParts];  // of the runs that all parts add up: the tile behind the last
-    __shared__ unsigned int keys[kParts];
+    __shared__ int64_t ends[kMostParts];  // of the runs that all parts add up: the tile behind the last
+    __shared__ unsigned int keys[kMostParts];
     grid_dependency_release();
     grid_dependency_wait();
-    const int tx = threadIdx.x % kPartThreads, ty = threadIdx.x / kPartThreads, lane = threadIdx.x & 31;
-    const int slabs = (c.groups + kPartThreads - 1) / kPartThreads, g = (int)(blockIdx.x % slabs) * kPartThreads + tx;
-    const int64_t first = (int64_t)(blockIdx.x / slabs) * kParts;
+    const int tx = threadIdx.x & (x - 1), ty = threadIdx.x / x, parts = kGradientThreads / x, lane = threadIdx.x & 31;
+    const int slabs = (c.groups + x - 1) / x, g = (int)(blockIdx.x % slabs) * x + tx;
+    const int64_t first = (int64_t)(blockIdx.x / slabs) * parts;
     {
         const int64_t t = first + ty, begin = t * c.tile, end = begin + c.tile;
         unsigned int key = (unsigned int)c.rows;
@@ -273,12 +361,15 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
             const bool leaves = key < (unsigned int)c.rows && c.keys[end] == key;
             starts = leaves && (c.keys[begin] != key || !begin || c.keys[begin - 1] != key);
         }
-        int64_t behind = t + 1;  // the first tile that does not begin with the run's key; 32 are asked at a time
-        while (starts) {
-            const int64_t at = (behind + lane + 1) * c.tile;
-            const unsigned int ended = __ballot_sync(0xffffffffu, at >= c.n || c.keys[at] != key);
-            behind += ended ? __ffs(ended) : 32;
-            if (ended) break;
+        int64_t behind = t + 1;  // the first tile that does not begin with the run's key; the lanes of a part ask for one each
+        const int asked = x < 32 ? x : 32, own = lane & (asked - 1);
+        for (bool open = starts; __any_sync(0xffffffffu, open);) {
+            const int64_t at = (behind + own + 1) * c.tile;
+            const unsigned int ended = __ballot_sync(0xffffffffu, open && (at >= c.n || c.keys[at] != key)) >> (lane - own) & (~0u >> (32 - asked));
+            if (open) {
+                behind += ended ? __ffs(ended) : asked;
+                open = !ended;
+            }
         }
         const bool few = behind - t <= kAhead;
         if (starts && few && g < c.groups) {
@@ -286,7 +377,7 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
 #pragma unroll
             for (int k = 0; k < G; ++k) sum[k] = 0.0f;
             add_shares<G>(sum, c, t, t, behind, g);
-            write_row<TOut, G>(c, out, key, g, sum);
+            write_row<SHIFTED>(c, out, key, g, sum);
         }
         if (tx == 0) {
             ends[ty] = starts && !few ? behind : -1;
@@ -294,15 +385,15 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
         }
     }
     __syncthreads();
-    for (int j = 0; j < kParts; ++j) {  // (all threads of the block alike)
+    for (int j = 0; j < parts; ++j) {  // (all threads of the block alike)
         const int64_t t = first + j, count = ends[j] - t;
         if (ends[j] < 0) continue;
         float sum[G];
 #pragma unroll
         for (int k = 0; k < G; ++k) sum[k] = 0.0f;
-        if (g < c.groups) add_shares<G>(sum, c, t, t + count * ty / kParts, t + count * (ty + 1) / kParts, g);
-        join_parts<G>(sum, part, tx, ty);
-        if (ty == 0 && g < c.groups) write_row<TOut, G>(c, out, keys[j], g, sum);
+        if (g < c.groups) add_shares<G>(sum, c, t, t + count * ty / parts, t + count * (ty + 1) / parts, g);
+        join_parts<G>(sum, part, x);
+        if (ty == 0 && g < c.groups) write_row<SHIFTED>(c, out, keys[j], g, sum);
     }
 }
 
@@ -311,9 +402,9 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
 // lists the positions that name the row and adds them up, in y parts that are joined in order.  What clears does so with
 // the bits of its own rows, from all tokens as well.  (Sorting them would take one block 13 us and the launches around it
 // 5, whatever the table.)
-constexpr int64_t kFewTokens = 1024;
+constexpr int64_t kFewTokens = 512;
 
-template <typename TIn, typename TOut, int G>
+template <typename TIn, typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kGradientThreads)
 gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ upstream, TOut *__restrict__ out, TempHeader *hdr) {
     grid_dependency_release();
@@ -321,24 +412,26 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
     __shared__ unsigned short list[kFewTokens];
     __shared__ float part[kGradientThreads * G];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (int)c.n;
-    if (blockIdx.x >= c.sum_blocks) {
-        const int64_t first = (blockIdx.x - c.sum_blocks) * c.clear_rows;  // clear_rows: 32 for each warp at most
+    // blocks that clear evenly between those that sum
+    const unsigned int block = (unsigned int)((unsigned long long)blockIdx.x * c.sum_blocks / gridDim.x);
+    if (block == (unsigned int)((blockIdx.x + 1ull) * c.sum_blocks / gridDim.x)) {
+        const int64_t first = (int64_t)(blockIdx.x - block) * c.clear_rows;  // clear_rows: 32 for each warp at most
         if (threadIdx.x < kGradientThreads / 32) bits[threadIdx.x] = 0u;
         __syncthreads();
         grid_dependency_wait();
         if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) hdr->wait_limit_hit = 0u;  // no wait can run out
         for (int i = threadIdx.x; i < n; i += kGradientThreads) {
-            const int64_t at = tokens[i] - first;
-            if (at >= 0 && at < c.clear_rows) atomicOr(bits + (at >> 5), 1u << (at & 31));
+            const int64_t token = tokens[i];
+            if (token >= first && token < first + c.clear_rows) atomicOr(bits + ((token - first) >> 5), 1u << ((token - first) & 31));
         }
         __syncthreads();
         for (int i = warp; i < c.clear_rows; i += kGradientThreads / 32)
-            if (first + i < c.rows && !(bits[i >> 5] >> (i & 31) & 1)) clear_rows<TOut, G>(c, out, first + i, 1u);
+            if (first + i < c.rows && !(bits[i >> 5] >> (i & 31) & 1)) clear_rows<SHIFTED, G>(c, out, first + i, 1u);
         return;
     }
     grid_dependency_wait();
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) hdr->wait_limit_hit = 0u;
-    const int i = (int)(blockIdx.x / c.slabs);
+    const int i = (int)(block / c.slabs);
     const int64_t token = tokens[i];
     if (token < 0 || token >= c.rows) return;
     for (int base = 0; base < n; base += kGradientThreads) {
@@ -359,32 +452,39 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
     if (earlier) return;
     __syncthreads();
     const int tx = threadIdx.x % kPartThreads, ty = threadIdx.x / kPartThreads;
-    const int g = (int)(blockIdx.x % c.slabs) * kPartThreads + tx;
+    constexpr int kFewAhead = SHIFTED ? 4 : 8;  // (shifted columns take twice the registers, which would cost blocks on an SM)
     const int begin = count * ty / kParts, end = count * (ty + 1) / kParts;
-    float sum[G];
+    const int64_t row = token * c.row_stride;
+    for (int first = (int)(block % c.slabs) * kPartThreads; first < c.groups; first += c.slabs * kPartThreads) {
+        const int g = first + tx;
+        float sum[G];
 #pragma unroll
-    for (int k = 0; k < G; ++k) sum[k] = 0.0f;
-    for (int r = begin; r < end && g < c.groups; r += kAhead) {
-        Group<TIn, G> in[kAhead];
+        for (int k = 0; k < G; ++k) sum[k] = 0.0f;
+        const TIn *from = upstream + column_of<SHIFTED, G>(out + row, g);
+        for (int r = begin; r < end && g < c.groups; r += kFewAhead) {
+            Columns<TIn, G, SHIFTED> in[kFewAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            in[j].clear();
-            if (r + j < end) in[j].load(upstream + list[r + j] * c.upstream_stride + (int64_t)g * G);
+            for (int j = 0; j < kFewAhead; ++j) {
+                in[j].clear();
+                if (r + j < end) in[j].load(from + list[r + j] * c.upstream_stride, c.extent);
+            }
+#pragma unroll
+            for (int j = 0; j < kFewAhead; ++j) {
+                const Group<TIn, G> x = in[j].get();
+#pragma unroll
+                for (int k = 0; k < G; ++k) sum[k] += x.get(k);
+            }
         }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-            for (int k = 0; k < G; ++k) sum[k] += in[j].get(k);
+        join_parts<G>(sum, part, kPartThreads);
+        if (ty == 0 && g < c.groups) write_row<SHIFTED>(c, out, (unsigned int)token, g, sum);
     }
-    join_parts<G>(sum, part, tx, ty);
-    if (ty == 0 && g < c.groups) write_row<TOut, G>(c, out, (unsigned int)token, g, sum);
 }
 
-// Sorted positions of a tile: enough blocks for the GPU, and shares of crossing runs that stay a small part of the
-// traffic.
-static int64_t gradient_tile(int64_t n) {
+// Sorted positions of a tile: enough blocks for the GPU (a narrow row leaves room for many tiles in one), and shares of
+// crossing runs that stay a small part of the traffic.
+static int64_t gradient_tile(int64_t n, int64_t width) {
     int64_t tile = 128;
-    while (tile > 16 && ceil_div(n, tile) < 148 * 3 / 2) tile /= 2;
+    while (tile > 16 && ceil_div(n, tile) * (width < 2048 ? width : 2048) < (int64_t)148 * 3 / 2 * 2048) tile /= 2;
     return tile;
 }
 
@@ -395,9 +495,9 @@ struct GradientLayout {
 static int gradient_layout(int64_t rows, int64_t width, int64_t n, GradientLayout &L) {
     if (rows < 0 || width < 0 || n < 0) return B200ALG_INVALID_ARGUMENT;
     if (rows > INT32_MAX || width > INT32_MAX || n > INT32_MAX) return B200ALG_TOO_LARGE;
-    L.tile = gradient_tile(n);
+    L.tile = gradient_tile(n, width);
     L.tiles = ceil_div(n, L.tile);
-    L.share_stride = round_up(width, 8);
+    L.share_stride = round_up(width + kShiftedGroup, 8) + 8;  // a shifted row has a group or two more
     const int rc = b200alg_radix_sort_temp_bytes(B200ALG_U32, n, 4, &L.sort_bytes);  // its part lies first, and with it its status word
     if (rc != B200ALG_OK) return rc;
     L.off_keys = round_up(L.sort_bytes, 256);
@@ -415,18 +515,22 @@ static int rows_to_clear(int64_t width, int bytes, int most) {
     return (int)(rows < kGradientThreads / 32 ? kGradientThreads / 32 : rows > most ? most : rows / (kGradientThreads / 32) * (kGradientThreads / 32));
 }
 
-template <typename TIn, typename TOut, int G>
+template <typename TIn, typename TOut, int G, bool SHIFTED>
 static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens, const GradientLayout &L, const void *upstream, void *out, void *temp) {
-    c.groups = (int)(c.width / G);
+    c.groups = (int)groups_in(c.width, G, SHIFTED);
+    c.extent = extent_of(upstream, c.n, c.width, c.upstream_stride, sizeof(TIn));
     char *t = (char *)temp;
     if (c.n <= kFewTokens) {
-        c.slabs = (int)ceil_div(c.groups, kPartThreads);
+        // columns of a position that different blocks take: as many as make some thousands of blocks
+        const int64_t slabs = ceil_div(c.groups, kPartThreads), most = ceil_div(2048, c.n ? c.n : 1);
+        c.slabs = (int)(slabs < most ? slabs : most);
         c.sum_blocks = c.n * c.slabs;
         c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 256);
-        const int64_t blocks = c.sum_blocks + (c.accumulate ? 0 : ceil_div(c.rows, c.clear_rows));
+        c.clear_blocks = c.accumulate ? 0 : ceil_div(c.rows, c.clear_rows);
+        const int64_t blocks = c.sum_blocks + c.clear_blocks;
         if (blocks > INT32_MAX) return B200ALG_TOO_LARGE;
         if (blocks)
-            B200ALG_CUDA_TRY(launch_dependent(gradient_few_kernel<TIn, TOut, G>, dim3((unsigned)blocks), dim3(kGradientThreads), 0, s, c, tokens,
+            B200ALG_CUDA_TRY(launch_dependent(gradient_few_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)blocks), dim3(kGradientThreads), 0, s, c, tokens,
                                               (const TIn *)upstream, (TOut *)out, (TempHeader *)temp));
         return B200ALG_OK;
     }
@@ -450,12 +554,13 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     c.early = one_launch;
     c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 1 << 20);
     c.clear_blocks = named ? ceil_div(c.rows, c.clear_rows) : 0;
-    if (c.sum_blocks + c.clear_blocks > INT32_MAX || ceil_div(c.tiles, kParts) * ceil_div(c.groups, kPartThreads) > INT32_MAX) return B200ALG_TOO_LARGE;
+    const int x = part_threads(c.groups);
+    const int64_t join_blocks = ceil_div(c.tiles, kGradientThreads / x) * ceil_div(c.groups, x);
+    if (c.sum_blocks + c.clear_blocks > INT32_MAX || join_blocks > INT32_MAX) return B200ALG_TOO_LARGE;
     const size_t smem = (size_t)c.y * (2 * c.tile + 3) * 4;  // (33 KB at most)
-    B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G>, dim3((unsigned)(c.sum_blocks + c.clear_blocks)), dim3(kGradientThreads), smem, s, c,
+    B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)(c.sum_blocks + c.clear_blocks)), dim3(kGradientThreads), smem, s, c,
                                       (const TIn *)upstream, (TOut *)out));
-    B200ALG_CUDA_TRY(launch_dependent(gradient_join_kernel<TOut, G>, dim3((unsigned)(ceil_div(c.tiles, kParts) * ceil_div(c.groups, kPartThreads))),
-                                      dim3(kGradientThreads), 0, s, c, (TOut *)out));
+    B200ALG_CUDA_TRY(launch_dependent(gradient_join_kernel<TOut, G, SHIFTED>, dim3((unsigned)join_blocks), dim3(kGradientThreads), 0, s, c, (TOut *)out, x));
     return B200ALG_OK;
 }
 
@@ -483,9 +588,10 @@ extern "C" int b200alg_embedding(void *stream, const void *table, int64_t rows, 
             using TIn = decltype(in);
             using TOut = decltype(to);
             constexpr int G = 32 / (sizeof(TIn) > sizeof(TOut) ? sizeof(TIn) : sizeof(TOut));
-            if (fits(G)) return run_lookup<TIn, TOut, G>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
-            if (fits(4)) return run_lookup<TIn, TOut, 4>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
-            return run_lookup<TIn, TOut, 1>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
+            if (fits(G)) return run_lookup<TIn, TOut, G, false>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
+            if constexpr (G == 16)
+                if (fits(8)) return run_lookup<TIn, TOut, 8, false>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
+            return run_lookup<TIn, TOut, kShiftedGroup, true>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
         });
     });
 }
@@ -526,8 +632,8 @@ extern "C" int b200alg_embedding_gradient(void *stream, const void *tokens, int6
             using TOut = decltype(to);
             constexpr int G = 16 / sizeof(TIn);
             if (groups_aligned(upstream, upstream_stride, n, width, ib, G) && groups_aligned(gradient, row_stride, rows, width, ob, G))
-                return run_gradient<TIn, TOut, G>(s, c, view, L, upstream, gradient, temp);
-            return run_gradient<TIn, TOut, 1>(s, c, view, L, upstream, gradient, temp);
+                return run_gradient<TIn, TOut, G, false>(s, c, view, L, upstream, gradient, temp);
+            return run_gradient<TIn, TOut, kShiftedGroup, true>(s, c, view, L, upstream, gradient, temp);
         });
     });
 }
