@@ -491,6 +491,7 @@ template <typename Call> static int with_row(int dtype, int experts, bool whole_
         }
         if (experts <= 16) return call(element, RowShape<1, 8, 2, 2>{});
         if (experts <= 64) return call(element, RowShape<1, 8, 8, 2>{});
+        if (experts <= 128) return call(element, RowShape<1, 8, 16, 2>{});
         if (experts <= 256) return call(element, RowShape<1, 8, 32, 2>{});
         return call(element, RowShape<1, 32, 32, 1>{});
     });
@@ -500,11 +501,12 @@ template <typename S> static BalanceCall balance_call(int64_t tokens, int64_t lo
     return BalanceCall{tokens, logits_stride, (int)experts, (int)choices, (const unsigned char *)mask, (int)experts / S::V};
 }
 
-// Blocks of a call: one for a few rows, then a cluster of them, and from about a megabyte on (0) as many as there is
-// work for.
-static int balance_cluster(int64_t tokens, int64_t experts) {
+// Blocks of a call: one for a few rows, then a cluster of them, and from where one is slower than two launches (0) as
+// many as there is work for.  In bf16 64 experts, us, cluster / two launches: 2048 tokens 6.6 / 7.2, 4096 8.9 / 7.6; rows
+// that do not lie on boundaries take longer: 1576 tokens of 99 experts in float 13.7 / 8.
+static int balance_cluster(int64_t tokens, int64_t experts, bool whole_groups) {
     const int64_t cells = tokens * experts;
-    return cells <= 4096 ? 1 : cells <= 1 << 18 ? kBalanceCluster : 0;
+    return cells <= 4096 ? 1 : cells <= (whole_groups ? 1 << 17 : 1 << 15) ? kBalanceCluster : 0;
 }
 
 // Resident blocks of a kernel on the whole GPU (asked once per context; `cache` is the kernel's own).
@@ -529,7 +531,7 @@ static int check_router(int64_t tokens, int64_t experts, int64_t choices, int64_
 }
 
 static int64_t balance_temp_bytes(int64_t experts, int64_t tokens) {
-    const int64_t blocks = balance_cluster(tokens, experts) ? 0 : kMostBalanceBlocks;
+    const int64_t blocks = balance_cluster(tokens, experts, false) ? 0 : kMostBalanceBlocks;
     return sizeof(TempHeader) + round_up(blocks * experts * 4, 256) + round_up(blocks * (experts + 1) * 4, 256);
 }
 
@@ -559,13 +561,13 @@ extern "C" int b200alg_balance_loss(void *stream, const void *logits, int64_t to
         return B200ALG_MISALIGNED;
     if (temp_bytes < balance_temp_bytes(experts, tokens)) return B200ALG_TEMP_TOO_SMALL;
     cudaStream_t s = (cudaStream_t)stream;
-    const int cluster = balance_cluster(tokens, experts);
     int blocks = 0;
     BalanceShares shares;
     shares.sums = (float *)((char *)temp + sizeof(TempHeader));
     shares.counts = (unsigned int *)((char *)temp + sizeof(TempHeader) + round_up(kMostBalanceBlocks * experts * 4, 256));
     const BalanceResult to{coefficient * experts / choices, loss, counts, probabilities};
     const bool whole = groups_aligned(logits, logits_stride, tokens, experts, bytes, 16 / bytes);
+    const int cluster = balance_cluster(tokens, experts, whole);
     const size_t smem = (size_t)padded_bins((int)experts) * (1 + kBalanceWarps) * 4 + (cluster ? (size_t)ceil_div(experts, cluster) * 8 : 0);
     rc = with_row(dtype, (int)experts, whole, [&](auto element, auto shape) -> int {
         using T = decltype(element);

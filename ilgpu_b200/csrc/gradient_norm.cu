@@ -20,7 +20,8 @@ constexpr int kMaxBlocks = 148 * kNormBlocksPerSm;  // partial sums of a launch
 constexpr int kMostViews = 1024;                    // of a launch: 30 KB of parameters
 constexpr int kMostSpan = 8;                        // chunks that a block takes one behind the other
 
-constexpr int kFewViews = 64;                       // of a launch with a short list: 2 KB of parameters cost the host 1 us less
+// of a launch with a shorter list, whose parameters (2 and 7 KB) cost the host less time: 1 us a launch with 64 views
+constexpr int kFewViews = 64, kSomeViews = 256;
 
 template <int MOST> struct ViewTable {
     const void *in[MOST];
@@ -430,6 +431,7 @@ extern "C" int b200alg_gradient_norm(void *stream, const void *const *views, con
     if (temp_bytes < norm_temp_bytes(count)) return B200ALG_TEMP_TOO_SMALL;
     const ViewLists l{views, nullptr, lengths, dtypes, nullptr, count};
     if (count <= kFewViews) return run_clip<kFewViews>((cudaStream_t)stream, l, norm, -1.0, temp);
+    if (count <= kSomeViews) return run_clip<kSomeViews>((cudaStream_t)stream, l, norm, -1.0, temp);
     return run_clip<kMostViews>((cudaStream_t)stream, l, norm, -1.0, temp);
 }
 
@@ -441,6 +443,7 @@ extern "C" int b200alg_gradient_scale(void *stream, const void *const *views, vo
     if ((uintptr_t)norm % 4) return B200ALG_MISALIGNED;
     const ViewLists l{views, outputs, lengths, dtypes, out_dtypes, count};
     if (count <= kFewViews) return run_scale<kFewViews>((cudaStream_t)stream, l, nullptr, 0, (float *)norm, max_norm);
+    if (count <= kSomeViews) return run_scale<kSomeViews>((cudaStream_t)stream, l, nullptr, 0, (float *)norm, max_norm);
     return run_scale<kMostViews>((cudaStream_t)stream, l, nullptr, 0, (float *)norm, max_norm);
 }
 
@@ -453,5 +456,6 @@ extern "C" int b200alg_gradient_clip(void *stream, const void *const *views, voi
     if (temp_bytes < norm_temp_bytes(count)) return B200ALG_TEMP_TOO_SMALL;
     const ViewLists l{views, outputs, lengths, dtypes, out_dtypes, count};
     if (count <= kFewViews) return run_clip<kFewViews>((cudaStream_t)stream, l, norm, max_norm, temp);
+    if (count <= kSomeViews) return run_clip<kSomeViews>((cudaStream_t)stream, l, norm, max_norm, temp);
     return run_clip<kMostViews>((cudaStream_t)stream, l, norm, max_norm, temp);
 }
