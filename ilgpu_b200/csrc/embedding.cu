@@ -13,7 +13,8 @@ namespace b200alg {
 
 // Where rows do not lie on boundaries that groups can be moved from and to whole, groups of four columns begin on the
 // boundaries of the OUTPUT row (the first and the last one of a row stick out of it), and are put together from the two
-// aligned words of the input that hold them.  SHIFTED below.  (One element at a time instead: XX.)
+// aligned words of the input that hold them.  SHIFTED below.  (One element at a time: 60001 rows of 1357
+// bf16 184 us instead of 79.)
 constexpr int kShiftedGroup = 4;
 
 // Extent of a matrix that is read: a word that overlaps it may be loaded whole (an aligned word lies in one page).

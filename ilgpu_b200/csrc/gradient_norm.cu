@@ -402,11 +402,29 @@ template <int MOST> static int run_scale(cudaStream_t s, const ViewLists &l, con
 
 // The norm, and with max_norm >= 0 the clipping by it.
 template <int MOST> static int run_clip(cudaStream_t s, const ViewLists &l, float *norm, double max_norm, void *temp) {
-    double *partial = (double *)((char *)temp + sizeof(TempHeader));
+    double *const partial = (double *)((char *)temp + sizeof(TempHeader));
     int sums = 0;
-    const int rc = run_partial<MOST>(s, l, max_norm >= 0.0, partial, &sums);
-    if (rc != B200ALG_OK) return rc;
-    if (max_norm >= 0.0) return run_scale<MOST>(s, l, partial, sums, norm, max_norm);
+    if (l.count <= MOST) {  // one table for both passes
+        ViewTable<MOST> t;
+        fill_table(t, l.in, l.out, l.lengths, l.in_types, l.out_types, 0, l.count);
+        if (t.views) {
+            sums = blocks_of(t);
+            double *to = partial;
+            void *arguments[] = {&t, &to};
+            B200ALG_CUDA_TRY(launch_with_table(max_norm >= 0.0 ? (const void *)norm_partial_kernel<MOST, true> : (const void *)norm_partial_kernel<MOST, false>,
+                                               sums, s, arguments));
+            if (max_norm >= 0.0) {
+                const double *from = partial;
+                void *scale_arguments[] = {&t, &from, &sums, &norm, &max_norm};
+                B200ALG_CUDA_TRY(launch_with_table((const void *)scale_kernel<MOST>, sums, s, scale_arguments));
+                return B200ALG_OK;
+            }
+        }
+    } else {
+        int rc = run_partial<MOST>(s, l, max_norm >= 0.0, partial, &sums);
+        if (rc == B200ALG_OK && max_norm >= 0.0 && sums) rc = run_scale<MOST>(s, l, partial, sums, norm, max_norm);
+        if (rc != B200ALG_OK || (max_norm >= 0.0 && sums)) return rc;
+    }
     B200ALG_CUDA_TRY(launch_dependent(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, (const double *)partial, sums, norm));
     return B200ALG_OK;
 }

@@ -246,7 +246,8 @@ int b200alg_run_length_encode(void *stream, const void *data, int64_t n, int dty
  * Element types are F32, F16 and BF16; sums are held in 32 bits or more, in an order that
  * depends on sizes only, and results are rounded once.  Token and expert indices are I32 or
  * I64.  Matrices are row-major with rows `*_stride` elements apart; what lies between the
- * width of a row and the next row is neither read nor written.  Outputs overlap no input
+ * width of a row and the next row is not written, and what it holds does not matter (a load
+ * may take in bytes beside a row that share an aligned 16 bytes with it).  Outputs overlap no input
  * (b200alg_gradient_clip and b200alg_gradient_scale may work in place).  At most 2^31 - 1
  * rows, columns and tokens (B200ALG_TOO_LARGE). */
 

@@ -16,9 +16,13 @@
 //   Histogram / HistogramUnchecked      HistogramLaunchers.tt:52-101
 //   operation structs                   ScanReduceOperations.tt, RadixSortOperations.tt
 //   ArrayView / ArrayView1D / Stride1D  Src/ILGPU/ArrayView.cs, Runtime/ArrayViews.tt, Stride.cs
+// The operators of a language model's training step (b200alg_embedding and what follows it) have no
+// counterpart there and take the same form.
 // There is no fallback path: every call ends in the CUDA library.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -28,6 +32,7 @@
 #include <stdexcept>
 #include <string>
 #include <type_traits>
+#include <vector>
 
 #include "b200alg.h"
 
@@ -474,6 +479,186 @@ inline void HistogramUnchecked(const Accelerator &accelerator, const Accelerator
     B200AlgException::ThrowIfFailed(b200alg_histogram(stream.StreamPtr(), view.BaseView.Pointer, view.StrideExtent(), view.Length,
                                                       DTypeOf<T>::value, TLocator::Locator, locator.Lo, locator.Hi, histogram.Pointer,
                                                       histogram.Length, DTypeOf<TBinType>::value, nullptr));
+}
+
+// ---- operators of a training step ------------------------------------------------------------------
+// Element types float, __half and __nv_bfloat16; indices int32_t and int64_t.
+template <typename T> struct ElementOf;
+template <> struct ElementOf<float> { static constexpr int value = B200ALG_F32; };
+template <> struct ElementOf<__half> { static constexpr int value = B200ALG_F16; };
+template <> struct ElementOf<__nv_bfloat16> { static constexpr int value = B200ALG_BF16; };
+
+// A matrix whose rows are dense and RowStride elements apart (ArrayView2D<T, Stride2D.DenseX>).
+template <typename T> struct ArrayView2D {
+    ArrayView<T> BaseView;
+    int64_t Rows = 0, Width = 0, RowStride = 0;
+    ArrayView2D() = default;
+    ArrayView2D(ArrayView<T> base, int64_t rows, int64_t width, int64_t rowStride = -1)
+        : BaseView(base), Rows(rows), Width(width), RowStride(rowStride < 0 ? width : rowStride) {
+        if (rows < 0 || width < 0 || RowStride < width || (rows && base.Length < (rows - 1) * RowStride + width))
+            throw ArgumentOutOfRangeException("extent");
+    }
+    bool IsValid() const { return BaseView.IsValid(); }
+};
+
+// One of a list of dense views of different element types.
+struct ElementView {
+    void *Pointer;
+    int64_t Length;
+    int DType;
+    template <typename T> ElementView(ArrayView<T> view) : Pointer(view.Pointer), Length(view.Length), DType(ElementOf<T>::value) {}
+};
+
+template <typename TTable, typename TIndex, typename TOut>
+using Embedding = std::function<void(const AcceleratorStream &, ArrayView2D<TTable>, ArrayView1D<TIndex>, ArrayView2D<TOut>, double)>;
+template <typename TTable, typename TIndex, typename TOut>
+inline Embedding<TTable, TIndex, TOut> CreateEmbedding(const Accelerator &accelerator) {
+    return [accelerator](const AcceleratorStream &stream, ArrayView2D<TTable> table, ArrayView1D<TIndex> tokens, ArrayView2D<TOut> output,
+                         double scale) {
+        if (!table.IsValid()) throw ArgumentNullException("table");
+        if (!tokens.IsValid()) throw ArgumentNullException("tokens");
+        if (!output.IsValid()) throw ArgumentNullException("output");
+        if (output.Width != table.Width || output.Rows < tokens.Length) throw ArgumentOutOfRangeException("output");
+        accelerator.Bind();
+        B200AlgException::ThrowIfFailed(b200alg_embedding(
+            stream.StreamPtr(), table.BaseView.Pointer, table.Rows, table.Width, table.RowStride, ElementOf<TTable>::value, tokens.BaseView.Pointer,
+            tokens.Length, tokens.StrideExtent(), DTypeOf<TIndex>::value, scale, output.BaseView.Pointer, output.RowStride, ElementOf<TOut>::value));
+    };
+}
+
+inline int64_t ComputeEmbeddingGradientTempStorageSize(const Accelerator &, int64_t rows, int64_t width, int64_t dataLength) {
+    int64_t bytes = 0;
+    B200AlgException::ThrowIfFailed(b200alg_embedding_gradient_temp_bytes(rows, width, dataLength, &bytes));
+    return detail::IntsFor(bytes);
+}
+template <typename TIndex, typename TUpstream, typename TTable>
+using EmbeddingGradient =
+    std::function<void(const AcceleratorStream &, ArrayView1D<TIndex>, ArrayView2D<TUpstream>, ArrayView2D<TTable>, ArrayView<int>, double)>;
+template <typename TIndex, typename TUpstream, typename TTable>
+inline EmbeddingGradient<TIndex, TUpstream, TTable> CreateEmbeddingGradient(const Accelerator &accelerator, bool accumulate = false) {
+    return [accelerator, accumulate](const AcceleratorStream &stream, ArrayView1D<TIndex> tokens, ArrayView2D<TUpstream> outputGradient,
+                                     ArrayView2D<TTable> tableGradient, ArrayView<int> temp, double scale) {
+        if (!tokens.IsValid()) throw ArgumentNullException("tokens");
+        if (!outputGradient.IsValid()) throw ArgumentNullException("outputGradient");
+        if (!tableGradient.IsValid()) throw ArgumentNullException("tableGradient");
+        if (outputGradient.Width != tableGradient.Width || outputGradient.Rows < tokens.Length) throw ArgumentOutOfRangeException("outputGradient");
+        detail::CheckTemp(temp, ComputeEmbeddingGradientTempStorageSize(accelerator, tableGradient.Rows, tableGradient.Width, tokens.Length));
+        accelerator.Bind();
+        B200AlgException::ThrowIfFailed(b200alg_embedding_gradient(
+            stream.StreamPtr(), tokens.BaseView.Pointer, tokens.Length, tokens.StrideExtent(), DTypeOf<TIndex>::value, outputGradient.BaseView.Pointer,
+            outputGradient.RowStride, ElementOf<TUpstream>::value, scale, tableGradient.BaseView.Pointer, tableGradient.Rows, tableGradient.Width,
+            tableGradient.RowStride, ElementOf<TTable>::value, accumulate ? 1 : 0, temp.Pointer, temp.LengthInBytes()));
+    };
+}
+
+namespace detail {
+struct ElementLists {
+    std::vector<const void *> in;
+    std::vector<void *> out;
+    std::vector<int64_t> lengths;
+    std::vector<int> types, out_types;
+    ElementLists(const std::vector<ElementView> &views, const std::vector<ElementView> *outputs) {
+        if (outputs && outputs->size() != views.size()) throw ArgumentOutOfRangeException("outputs");
+        for (size_t i = 0; i < views.size(); ++i) {
+            in.push_back(views[i].Pointer);
+            lengths.push_back(views[i].Length);
+            types.push_back(views[i].DType);
+            if (!outputs) continue;
+            if ((*outputs)[i].Length != views[i].Length) throw ArgumentOutOfRangeException("outputs");
+            out.push_back((*outputs)[i].Pointer);
+            out_types.push_back((*outputs)[i].DType);
+        }
+    }
+};
+}  // namespace detail
+
+inline int64_t ComputeGradientNormTempStorageSize(const Accelerator &, int64_t numViews) {
+    int64_t bytes = 0;
+    B200AlgException::ThrowIfFailed(b200alg_gradient_norm_temp_bytes(numViews, &bytes));
+    return detail::IntsFor(bytes);
+}
+inline void GradientNorm(const Accelerator &accelerator, const AcceleratorStream &stream, const std::vector<ElementView> &views, ArrayView<float> norm,
+                         ArrayView<int> temp) {
+    if (!norm.IsValid()) throw ArgumentNullException("norm");
+    if (norm.Length < 1) throw ArgumentOutOfRangeException("norm");
+    detail::CheckTemp(temp, ComputeGradientNormTempStorageSize(accelerator, (int64_t)views.size()));
+    const detail::ElementLists l(views, nullptr);
+    accelerator.Bind();
+    B200AlgException::ThrowIfFailed(b200alg_gradient_norm(stream.StreamPtr(), l.in.data(), l.lengths.data(), l.types.data(), (int64_t)views.size(),
+                                                          norm.Pointer, temp.Pointer, temp.LengthInBytes()));
+}
+// outputs == nullptr: in place.
+inline void GradientClip(const Accelerator &accelerator, const AcceleratorStream &stream, const std::vector<ElementView> &views,
+                         const std::vector<ElementView> *outputs, double maxNorm, ArrayView<float> norm, ArrayView<int> temp) {
+    if (!norm.IsValid()) throw ArgumentNullException("norm");
+    if (norm.Length < 1) throw ArgumentOutOfRangeException("norm");
+    if (!(maxNorm >= 0.0)) throw ArgumentOutOfRangeException("maxNorm");
+    detail::CheckTemp(temp, ComputeGradientNormTempStorageSize(accelerator, (int64_t)views.size()));
+    const detail::ElementLists l(views, outputs);
+    accelerator.Bind();
+    B200AlgException::ThrowIfFailed(b200alg_gradient_clip(stream.StreamPtr(), l.in.data(), outputs ? l.out.data() : nullptr, l.lengths.data(),
+                                                          l.types.data(), outputs ? l.out_types.data() : nullptr, (int64_t)views.size(), maxNorm,
+                                                          norm.Pointer, temp.Pointer, temp.LengthInBytes()));
+}
+// By a norm that is in device memory already.
+inline void GradientScale(const Accelerator &accelerator, const AcceleratorStream &stream, const std::vector<ElementView> &views,
+                          const std::vector<ElementView> *outputs, double maxNorm, ArrayView<float> norm) {
+    if (!norm.IsValid()) throw ArgumentNullException("norm");
+    if (norm.Length < 1) throw ArgumentOutOfRangeException("norm");
+    if (!(maxNorm >= 0.0)) throw ArgumentOutOfRangeException("maxNorm");
+    const detail::ElementLists l(views, outputs);
+    accelerator.Bind();
+    B200AlgException::ThrowIfFailed(b200alg_gradient_scale(stream.StreamPtr(), l.in.data(), outputs ? l.out.data() : nullptr, l.lengths.data(),
+                                                           l.types.data(), outputs ? l.out_types.data() : nullptr, (int64_t)views.size(),
+                                                           norm.Pointer, maxNorm));
+}
+
+inline int64_t ComputeBalanceLossTempStorageSize(const Accelerator &, int64_t numExperts, int64_t dataLength) {
+    int64_t bytes = 0;
+    B200AlgException::ThrowIfFailed(b200alg_balance_loss_temp_bytes(numExperts, dataLength, &bytes));
+    return detail::IntsFor(bytes);
+}
+namespace detail {
+inline void CheckRouter(int64_t tokens, int64_t experts, const ArrayView<uint8_t> &mask, const ArrayView<int32_t> &counts) {
+    if (mask.IsValid() && mask.Length < tokens) throw ArgumentOutOfRangeException("mask");
+    if (!counts.IsValid()) throw ArgumentNullException("counts");
+    if (counts.Length < experts + 1) throw ArgumentOutOfRangeException("counts");
+}
+}  // namespace detail
+// mask: a byte per token, or an invalid view: all tokens count.
+template <typename T, typename TIndex>
+inline void BalanceLoss(const Accelerator &accelerator, const AcceleratorStream &stream, ArrayView2D<T> logits, ArrayView2D<TIndex> experts,
+                        ArrayView<uint8_t> mask, double coefficient, ArrayView<float> loss, ArrayView<int32_t> counts, ArrayView<float> probabilities,
+                        ArrayView<int> temp) {
+    if (!logits.IsValid()) throw ArgumentNullException("logits");
+    if (!experts.IsValid()) throw ArgumentNullException("experts");
+    if (experts.Rows != logits.Rows) throw ArgumentOutOfRangeException("experts");
+    detail::CheckRouter(logits.Rows, logits.Width, mask, counts);
+    if (!loss.IsValid()) throw ArgumentNullException("loss");
+    if (loss.Length < 1) throw ArgumentOutOfRangeException("loss");
+    if (!probabilities.IsValid()) throw ArgumentNullException("probabilities");
+    if (probabilities.Length < logits.Width) throw ArgumentOutOfRangeException("probabilities");
+    detail::CheckTemp(temp, ComputeBalanceLossTempStorageSize(accelerator, logits.Width, logits.Rows));
+    accelerator.Bind();
+    B200AlgException::ThrowIfFailed(b200alg_balance_loss(
+        stream.StreamPtr(), logits.BaseView.Pointer, logits.Rows, logits.Width, logits.RowStride, ElementOf<T>::value, experts.BaseView.Pointer,
+        experts.Width, experts.RowStride, DTypeOf<TIndex>::value, mask.Pointer, coefficient, loss.Pointer, counts.Pointer, probabilities.Pointer,
+        temp.Pointer, temp.LengthInBytes()));
+}
+template <typename T>
+inline void BalanceLossGradient(const Accelerator &accelerator, const AcceleratorStream &stream, ArrayView2D<T> logits, ArrayView<uint8_t> mask,
+                                ArrayView<int32_t> counts, int64_t choices, double coefficient, ArrayView<float> lossGradient,
+                                ArrayView2D<T> logitsGradient, bool accumulate = false) {
+    if (!logits.IsValid()) throw ArgumentNullException("logits");
+    if (!logitsGradient.IsValid()) throw ArgumentNullException("logitsGradient");
+    if (logitsGradient.Rows != logits.Rows || logitsGradient.Width != logits.Width) throw ArgumentOutOfRangeException("logitsGradient");
+    detail::CheckRouter(logits.Rows, logits.Width, mask, counts);
+    if (!lossGradient.IsValid()) throw ArgumentNullException("lossGradient");
+    if (lossGradient.Length < 1) throw ArgumentOutOfRangeException("lossGradient");
+    accelerator.Bind();
+    B200AlgException::ThrowIfFailed(b200alg_balance_loss_gradient(
+        stream.StreamPtr(), logits.BaseView.Pointer, logits.Rows, logits.Width, logits.RowStride, ElementOf<T>::value, mask.Pointer, counts.Pointer,
+        choices, coefficient, lossGradient.Pointer, logitsGradient.BaseView.Pointer, logitsGradient.RowStride, accumulate ? 1 : 0));
 }
 
 }  // namespace Algorithms

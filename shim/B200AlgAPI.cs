@@ -63,6 +63,34 @@ namespace ILGPU.Runtime.Cuda
             IntPtr stream, IntPtr data, long n, int dtype, IntPtr outCount, IntPtr temp, long tempBytes);
 
         [LibraryImport(LibName)] internal static partial int b200alg_device_status(IntPtr stream, IntPtr temp);
+
+        // operators of a training step (no counterpart in ILGPU.Algorithms); views, lengths, dtypes: host arrays
+        [LibraryImport(LibName)] internal static partial int b200alg_embedding(
+            IntPtr stream, IntPtr table, long rows, long width, long rowStride, int dtype, IntPtr tokens, long n,
+            long tokenStride, int tokenDtype, double scale, IntPtr output, long outStride, int outDtype);
+        [LibraryImport(LibName)] internal static partial int b200alg_embedding_gradient_temp_bytes(long rows, long width, long n, out long bytes);
+        [LibraryImport(LibName)] internal static partial int b200alg_embedding_gradient(
+            IntPtr stream, IntPtr tokens, long n, long tokenStride, int tokenDtype, IntPtr upstream, long upstreamStride,
+            int upstreamDtype, double scale, IntPtr gradient, long rows, long width, long rowStride, int dtype,
+            int accumulate, IntPtr temp, long tempBytes);
+        [LibraryImport(LibName)] internal static partial int b200alg_gradient_norm_temp_bytes(long count, out long bytes);
+        [LibraryImport(LibName)] internal static partial int b200alg_gradient_norm(
+            IntPtr stream, IntPtr* views, long* lengths, int* dtypes, long count, IntPtr norm, IntPtr temp, long tempBytes);
+        [LibraryImport(LibName)] internal static partial int b200alg_gradient_scale(
+            IntPtr stream, IntPtr* views, IntPtr* outputs, long* lengths, int* dtypes, int* outDtypes, long count,
+            IntPtr norm, double maxNorm);
+        [LibraryImport(LibName)] internal static partial int b200alg_gradient_clip(
+            IntPtr stream, IntPtr* views, IntPtr* outputs, long* lengths, int* dtypes, int* outDtypes, long count,
+            double maxNorm, IntPtr norm, IntPtr temp, long tempBytes);
+        [LibraryImport(LibName)] internal static partial int b200alg_balance_loss_temp_bytes(long experts, long tokens, out long bytes);
+        [LibraryImport(LibName)] internal static partial int b200alg_balance_loss(
+            IntPtr stream, IntPtr logits, long tokens, long experts, long logitsStride, int dtype, IntPtr chosen,
+            long choices, long chosenStride, int chosenDtype, IntPtr maskOrNull, double coefficient, IntPtr loss,
+            IntPtr counts, IntPtr probabilities, IntPtr temp, long tempBytes);
+        [LibraryImport(LibName)] internal static partial int b200alg_balance_loss_gradient(
+            IntPtr stream, IntPtr logits, long tokens, long experts, long logitsStride, int dtype, IntPtr maskOrNull,
+            IntPtr counts, long choices, double coefficient, IntPtr lossGradient, IntPtr gradient, long gradientStride,
+            int accumulate);
 #else
         [DllImport(LibName)] internal static extern int b200alg_version();
         [DllImport(LibName)] internal static extern IntPtr b200alg_status_string(int status);
@@ -87,6 +115,34 @@ namespace ILGPU.Runtime.Cuda
             IntPtr stream, IntPtr input, long stride, long n, int inDtype, int locator, double lo, double hi,
             IntPtr bins, long numBins, int binDtype, IntPtr overflowOrNull);
         [DllImport(LibName)] internal static extern int b200alg_device_status(IntPtr stream, IntPtr temp);
+
+        // operators of a training step (no counterpart in ILGPU.Algorithms); views, lengths, dtypes: host arrays
+        [DllImport(LibName)] internal static extern int b200alg_embedding(
+            IntPtr stream, IntPtr table, long rows, long width, long rowStride, int dtype, IntPtr tokens, long n,
+            long tokenStride, int tokenDtype, double scale, IntPtr output, long outStride, int outDtype);
+        [DllImport(LibName)] internal static extern int b200alg_embedding_gradient_temp_bytes(long rows, long width, long n, out long bytes);
+        [DllImport(LibName)] internal static extern int b200alg_embedding_gradient(
+            IntPtr stream, IntPtr tokens, long n, long tokenStride, int tokenDtype, IntPtr upstream, long upstreamStride,
+            int upstreamDtype, double scale, IntPtr gradient, long rows, long width, long rowStride, int dtype,
+            int accumulate, IntPtr temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int b200alg_gradient_norm_temp_bytes(long count, out long bytes);
+        [DllImport(LibName)] internal static extern int b200alg_gradient_norm(
+            IntPtr stream, IntPtr* views, long* lengths, int* dtypes, long count, IntPtr norm, IntPtr temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int b200alg_gradient_scale(
+            IntPtr stream, IntPtr* views, IntPtr* outputs, long* lengths, int* dtypes, int* outDtypes, long count,
+            IntPtr norm, double maxNorm);
+        [DllImport(LibName)] internal static extern int b200alg_gradient_clip(
+            IntPtr stream, IntPtr* views, IntPtr* outputs, long* lengths, int* dtypes, int* outDtypes, long count,
+            double maxNorm, IntPtr norm, IntPtr temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int b200alg_balance_loss_temp_bytes(long experts, long tokens, out long bytes);
+        [DllImport(LibName)] internal static extern int b200alg_balance_loss(
+            IntPtr stream, IntPtr logits, long tokens, long experts, long logitsStride, int dtype, IntPtr chosen,
+            long choices, long chosenStride, int chosenDtype, IntPtr maskOrNull, double coefficient, IntPtr loss,
+            IntPtr counts, IntPtr probabilities, IntPtr temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int b200alg_balance_loss_gradient(
+            IntPtr stream, IntPtr logits, long tokens, long experts, long logitsStride, int dtype, IntPtr maskOrNull,
+            IntPtr counts, long choices, double coefficient, IntPtr lossGradient, IntPtr gradient, long gradientStride,
+            int accumulate);
 #endif
     }
 }

@@ -12,6 +12,7 @@ namespace ILGPU.Runtime.Cuda
     internal enum B200AlgDType : int
     {
         I8 = 0, U8 = 1, I16 = 2, U16 = 3, I32 = 4, U32 = 5, I64 = 6, U64 = 7, F16 = 8, F32 = 9, F64 = 10,
+        BF16 = 11,  // the operators of a training step only
     }
 
     /// <summary>b200alg_op.</summary>
