@@ -537,6 +537,18 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     }
     unsigned int *keys = (unsigned int *)(t + L.off_keys), *positions = (unsigned int *)(t + L.off_positions);
     unsigned char *named = c.accumulate ? nullptr : (unsigned char *)(t + L.off_named);
+    c.keys = keys, c.positions = positions, c.named = named;
+    c.tile = L.tile, c.tiles = L.tiles;
+    c.shares = (float *)(t + L.off_shares), c.share_stride = L.share_stride;
+    for (c.x = 8; c.x < kGradientThreads && c.x < c.groups; c.x *= 2) {}
+    c.y = kGradientThreads / c.x;
+    c.slabs = (int)ceil_div(c.groups, c.x);
+    c.sum_blocks = ceil_div(c.tiles, c.y) * c.slabs;
+    c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 1 << 20);
+    c.clear_blocks = named ? ceil_div(c.rows, c.clear_rows) : 0;
+    const int x = part_threads(c.groups);
+    const int64_t join_blocks = ceil_div(c.tiles, kGradientThreads / x) * ceil_div(c.groups, x);
+    if (c.sum_blocks + c.clear_blocks > INT32_MAX || join_blocks > INT32_MAX) return B200ALG_TOO_LARGE;
     const int64_t cap = (int64_t)sm_count() * 8;
     auto some = [&](int64_t want) { return dim3((unsigned)(want < cap ? want : cap)); };
     if (named)
@@ -545,19 +557,7 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     bool one_launch = false;
     const int rc = sort_with_positions(s, keys, positions, c.n, temp, L.sort_bytes, &one_launch);
     if (rc != B200ALG_OK) return rc;
-    c.keys = keys, c.positions = positions, c.named = named;
-    c.tile = L.tile, c.tiles = L.tiles;
-    c.shares = (float *)(t + L.off_shares), c.share_stride = L.share_stride;
-    for (c.x = 8; c.x < kGradientThreads && c.x < c.groups; c.x *= 2) {}
-    c.y = kGradientThreads / c.x;
-    c.slabs = (int)ceil_div(c.groups, c.x);
-    c.sum_blocks = ceil_div(c.tiles, c.y) * c.slabs;
     c.early = one_launch;
-    c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 1 << 20);
-    c.clear_blocks = named ? ceil_div(c.rows, c.clear_rows) : 0;
-    const int x = part_threads(c.groups);
-    const int64_t join_blocks = ceil_div(c.tiles, kGradientThreads / x) * ceil_div(c.groups, x);
-    if (c.sum_blocks + c.clear_blocks > INT32_MAX || join_blocks > INT32_MAX) return B200ALG_TOO_LARGE;
     const size_t smem = (size_t)c.y * (2 * c.tile + 3) * 4;  // (33 KB at most)
     B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)(c.sum_blocks + c.clear_blocks)), dim3(kGradientThreads), smem, s, c,
                                       (const TIn *)upstream, (TOut *)out));

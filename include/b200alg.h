@@ -270,7 +270,8 @@ int b200alg_embedding_gradient(void *stream, const void *tokens, int64_t n, int6
 
 /* norm[0] (float, device) = sqrt(sum of x^2) over all elements of `count` dense views.  The
  * lists (views, lengths, dtypes) are host memory and are not looked at after return; a view
- * may be empty, and no view at all has norm 0.  Squares that 32 bits do not hold are taken in
+ * may be empty, and no view at all has norm 0; a view that is listed twice counts twice (and
+ * cannot be clipped in place).  Squares that 32 bits do not hold are taken in
  * 64: the norm is right wherever it is a float itself.  At most 2^38 elements in all. */
 int b200alg_gradient_norm_temp_bytes(int64_t count, int64_t *out_bytes);
 int b200alg_gradient_norm(void *stream, const void *const *views, const int64_t *lengths, const int *dtypes,

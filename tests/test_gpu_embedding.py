@@ -111,6 +111,16 @@ def test_lookup_past_32_bits_of_elements(accelerator):
     assert not bool(out[:, 1:-1].any())
 
 
+def test_lookup_of_more_groups_than_one_launch_counts(accelerator):
+    n = (1 << 30) + 5_000
+    table = torch.tensor([[1.0, -1.0], [2.0, -2.0], [3.0, -3.0]], dtype=torch.bfloat16, device="cuda")
+    tokens = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(5).sub_(1)
+    out = torch.full((n, 2), 7.0, dtype=torch.bfloat16, device="cuda")
+    accelerator.CreateEmbedding()(None, table, tokens, out)
+    want = torch.where(tokens > 2, 0, tokens + 1).to(torch.bfloat16)
+    assert torch.equal(out[:, 0], want) and torch.equal(out[:, 1], -want)
+
+
 def _gradient(acc, tokens, upstream, out, scale=1.0, accumulate=False, stream=None):
     temp = acc.Allocate1D(acc.ComputeEmbeddingGradientTempStorageSize(out.shape[0], out.shape[1], tokens.numel()), torch.int32)
     temp.fill_(-1)  # whatever was there
@@ -121,7 +131,8 @@ def _gradient(acc, tokens, upstream, out, scale=1.0, accumulate=False, stream=No
 
 GRADIENT_SHAPES = [  # tokens, rows, width: one token, tiles of every length, runs over several tiles, wide and narrow rows
     (1, 1, 1), (1, 40, 8), (2, 3, 5), (15, 4, 64), (16, 100, 64), (17, 3, 33), (129, 9, 48), (300, 2000, 768), (2_367, 31, 40), (2_368, 5, 8),
-    (4_737, 700, 129), (20_000, 37, 24), (19_001, 5000, 64), (500, 300, 4_100),
+    (4_737, 700, 129), (20_000, 37, 24), (19_001, 5000, 64), (500, 300, 4_100), (512, 90, 72), (513, 90, 72), (5_000, 30_000, 256), (60_000, 9, 16),
+    (3_000, 50_000, 33), (10_000, 77, 2_051),
 ]
 
 
