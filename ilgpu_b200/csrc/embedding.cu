@@ -355,21 +355,27 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
     const int64_t first = (int64_t)(blockIdx.x / slabs) * parts;
     {
         const int64_t t = first + ty, begin = t * c.tile, end = begin + c.tile;
-        unsigned int key = (unsigned int)c.rows;
-        bool starts = false;  // whether a run begins in the tile and leaves it
-        if (end < c.n) {
-            key = c.keys[end - 1];
-            const bool leaves = key < (unsigned int)c.rows && c.keys[end] == key;
-            starts = leaves && (c.keys[begin] != key || !begin || c.keys[begin - 1] != key);
-        }
-        int64_t behind = t + 1;  // the first tile that does not begin with the run's key; the lanes of a part ask for one each
+        const bool there = end < c.n;
+        const unsigned int key = there ? c.keys[end - 1] : (unsigned int)c.rows, next = there ? c.keys[end] : 0u;
+        const unsigned int first_key = there ? c.keys[begin] : 0u, before = there && begin ? c.keys[begin - 1] : ~0u;
+        // whether a run begins in the tile and leaves it
+        const bool starts = there && key < (unsigned int)c.rows && next == key && (first_key != key || before != key);
+        // The first tile that does not begin with the run's key.  The lanes of a part ask at equal steps, which grow until
+        // one is past it and shrink again from there.
+        int64_t behind = t + 1, step = 1;
         const int asked = x < 32 ? x : 32, own = lane & (asked - 1);
         for (bool open = starts; __any_sync(0xffffffffu, open);) {
-            const int64_t at = (behind + own + 1) * c.tile;
+            const int64_t at = (behind + (own + 1) * step) * c.tile;
             const unsigned int ended = __ballot_sync(0xffffffffu, open && (at >= c.n || c.keys[at] != key)) >> (lane - own) & (~0u >> (32 - asked));
-            if (open) {
-                behind += ended ? __ffs(ended) : asked;
-                open = !ended;
+            if (!open) continue;
+            if (!ended) {
+                behind += asked * step;
+                step *= asked;
+            } else {
+                behind += (__ffs(ended) - 1) * step;
+                open = step > 1;
+                if (open) step /= asked;
+                else ++behind;
             }
         }
         const bool few = behind - t <= kAhead;
