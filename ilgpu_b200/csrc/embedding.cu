@@ -471,15 +471,13 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
         for (int r = begin; r < end && g < c.groups; r += kFewAhead) {
             Columns<TIn, G, SHIFTED> in[kFewAhead];
 #pragma unroll
-            for (int j = 0; j < kFewAhead; ++j) {
-                in[j].clear();
-                if (r + j < end) in[j].load(from + list[r + j] * c.upstream_stride, c.extent);
-            }
+            for (int j = 0; j < kFewAhead; ++j)  // (one load behind the other, without a branch between them)
+                in[j].load(from + list[r + j < end ? r + j : end - 1] * c.upstream_stride, c.extent);
 #pragma unroll
             for (int j = 0; j < kFewAhead; ++j) {
                 const Group<TIn, G> x = in[j].get();
 #pragma unroll
-                for (int k = 0; k < G; ++k) sum[k] += x.get(k);
+                for (int k = 0; k < G; ++k) sum[k] += r + j < end ? x.get(k) : 0.0f;
             }
         }
         join_parts<G>(sum, part, kPartThreads);
