@@ -439,12 +439,18 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
     grid_dependency_wait();
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) hdr->wait_limit_hit = 0u;
     const int i = (int)(block / c.slabs);
+    int64_t some[kFewTokens / kGradientThreads];  // this thread's share of the tokens, all under way at once
+#pragma unroll
+    for (int u = 0; u < kFewTokens / kGradientThreads; ++u) {
+        const int j = u * kGradientThreads + (int)threadIdx.x;
+        some[u] = j < n ? tokens[j] : -1;
+    }
     const int64_t token = tokens[i];
     if (token < 0 || token >= c.rows) return;
-    for (int base = 0; base < n; base += kGradientThreads) {
-        const int j = base + (int)threadIdx.x;
-        const unsigned int same = __ballot_sync(0xffffffffu, j < n && tokens[j] == token);
-        if (lane == 0 && base + warp * 32 < kFewTokens) bits[base / 32 + warp] = same;
+#pragma unroll
+    for (int u = 0; u < kFewTokens / kGradientThreads; ++u) {
+        const unsigned int same = __ballot_sync(0xffffffffu, some[u] == token);
+        if (lane == 0) bits[u * (kGradientThreads / 32) + warp] = same;
     }
     __syncthreads();
     const int words = (n + 31) / 32;
