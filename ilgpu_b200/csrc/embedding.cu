@@ -148,7 +148,8 @@ static int run_lookup(cudaStream_t s, const void *table, int64_t rows, int64_t w
 // tile.  A run of equal tokens inside a tile is written at once; a tile's share of a run that crosses its border goes to
 // temp, and gradient_join_kernel adds the shares up in order.  Rows that no token names, which are most of a large
 // table, are cleared by the other blocks of the same launch.  They know them from a byte per row and need not wait for the
-// sort, so that its time passes behind them.
+// sort, so that its time passes behind them.  Memory is the bound: 131072 rows of 4096 bf16 into 128000 rows of float take
+// 518 us, 3.2 GB at 6.0 TB/s; 16384 of 2048 into 32000 take 67, 55 of them in this kernel at 6.0 TB/s.
 constexpr int kGradientThreads = 256;
 constexpr int kAhead = 8;      // rows, or shares, that a thread has in flight
 

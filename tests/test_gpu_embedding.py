@@ -132,7 +132,7 @@ def _gradient(acc, tokens, upstream, out, scale=1.0, accumulate=False, stream=No
 GRADIENT_SHAPES = [  # tokens, rows, width: one token, tiles of every length, runs over several tiles, wide and narrow rows
     (1, 1, 1), (1, 40, 8), (2, 3, 5), (15, 4, 64), (16, 100, 64), (17, 3, 33), (129, 9, 48), (300, 2000, 768), (2_367, 31, 40), (2_368, 5, 8),
     (4_737, 700, 129), (20_000, 37, 24), (19_001, 5000, 64), (500, 300, 4_100), (512, 90, 72), (513, 90, 72), (5_000, 30_000, 256), (60_000, 9, 16),
-    (3_000, 50_000, 33), (10_000, 77, 2_051),
+    (3_000, 50_000, 33), (10_000, 77, 2_051), (2_000_003, 5_000, 8),
 ]
 
 
@@ -173,19 +173,21 @@ def test_gradient_added_to_what_is_there(accelerator, types, n, rows, width, kin
 def test_gradient_in_strided_views(accelerator, types, width, stride, offset, out_stride, out_offset):
     source, target = (TYPES[t] for t in types.split())
     gen = torch.Generator(device="cuda").manual_seed(width + stride)
-    n, rows = 700, 150
-    _, upstream = _matrix(gen, n + 2, width, source, stride, offset)
-    flat, out = _matrix(gen, rows, width, target, out_stride, out_offset)
-    tokens = _tokens(gen, n, rows, "outside", torch.int32, stride=2)
-    before = flat.clone()
-    _gradient(accelerator, tokens, upstream, out, 3.0)
-    assert_within(out, *embedding_gradient(tokens, upstream, 3.0, rows, target))
-    _same_gaps(flat, out, out_stride, out_offset, before)
+    rows = 150
+    for n in (300, 700):  # with and without a sort
+        _, upstream = _matrix(gen, n + 2, width, source, stride, offset)
+        flat, out = _matrix(gen, rows, width, target, out_stride, out_offset)
+        tokens = _tokens(gen, n, rows, "outside", torch.int32, stride=2)
+        before = flat.clone()
+        _gradient(accelerator, tokens, upstream, out, 3.0)
+        assert_within(out, *embedding_gradient(tokens, upstream, 3.0, rows, target))
+        _same_gaps(flat, out, out_stride, out_offset, before)
 
 
-def test_upstream_rows_without_a_row_of_the_table_are_not_read(accelerator):
-    upstream = torch.full((300, 24), float("nan"), device="cuda")
-    tokens = torch.full((300,), -1, dtype=torch.int64, device="cuda")
+@pytest.mark.parametrize("n", [300, 3_000])
+def test_upstream_rows_without_a_row_of_the_table_are_not_read(accelerator, n):
+    upstream = torch.full((n, 24), float("nan"), device="cuda")
+    tokens = torch.full((n,), -1, dtype=torch.int64, device="cuda")
     upstream[7], tokens[7] = 2.0, 4
     out = torch.empty(6, 24, device="cuda")
     _gradient(accelerator, tokens, upstream, out)
@@ -213,6 +215,19 @@ def test_gradient_bits_do_not_change(accelerator):
         again = torch.empty_like(first)
         _gradient(accelerator, tokens, upstream, again)
         assert torch.equal(first, again)
+
+
+@pytest.mark.parametrize("n", [400, 6_000])
+def test_what_is_not_finite_stays_in_its_row_and_column(accelerator, n):
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    upstream = torch.randn(n, 37, generator=gen, device="cuda")
+    tokens = torch.randint(0, 50, (n,), generator=gen, device="cuda")
+    upstream[7, 5], upstream[9, 36], upstream[11, 0] = float("nan"), float("inf"), -float("inf")
+    out = torch.empty(50, 37, device="cuda")
+    _gradient(accelerator, tokens, upstream, out)
+    exact, bound = embedding_gradient(tokens, upstream, 1.0, 50, torch.float32)
+    assert_within(out, exact, torch.where(bound.isfinite(), bound, 0.0))
+    assert int((~out.isfinite()).sum()) == 3
 
 
 def test_gradient_is_the_lookups(accelerator):
