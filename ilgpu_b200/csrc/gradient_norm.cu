@@ -33,6 +33,7 @@ template <int MOST> struct ViewTable {
     unsigned char in_type[MOST], out_type[MOST];
     int views;
     int span;
+    int in_place;  // whether all of them are
 };
 static_assert(sizeof(ViewTable<kMostViews>) <= 31 << 10, "fits a kernel's parameters");
 
@@ -48,11 +49,13 @@ static int64_t fill_table(ViewTable<MOST> &t, const void *const *in, void *const
     int64_t i = first;
     unsigned int chunks = 0;
     t.views = 0;
+    t.in_place = 1;
     for (; i < views && t.views < MOST; ++i) {
         if (!lengths[i]) continue;
         const int v = t.views++;
         t.in[v] = in[i];
         t.out[v] = out ? out[i] : (void *)in[i];
+        if (t.out[v] != t.in[v]) t.in_place = 0;
         t.length[v] = lengths[i];
         t.chunk[v] = chunks;
         t.in_type[v] = (unsigned char)in_types[i];
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_consta
     bool more = at.enter();
     grid_dependency_wait();
     Part next;
-    if (more) load_part<false>(next, t, at);
+    if (more) load_part<false>(next, t, at);  // (one chunk in vain where nothing is to be done)
     float whole;
     if (partial) {
         whole = norm_of(partial, count);
@@ -308,11 +311,14 @@ __global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_consta
         whole = *norm;
     }
     const float factor = factor_of(whole, max_norm);
+    if (factor == 1.0f && t.in_place) return;
+    auto changes = [&](int view) { return factor != 1.0f || t.in[view] != t.out[view]; };  // else it is neither read nor written
     while (more) {
         const Part part = next;
         more = at.next();
-        if (more) load_part<false>(next, t, at);
-        if (factor == 1.0f && t.in[part.view] == t.out[part.view]) continue;
+        if (more && changes(at.view)) load_part<false>(next, t, at);
+        else next.view = at.view;
+        if (!changes(part.view)) continue;
         switch (part.type) {
         case B200ALG_F32: scale_part_from<float>(part, t, factor); break;
         case B200ALG_F16: scale_part_from<__half>(part, t, factor); break;

@@ -112,6 +112,18 @@ def test_clip_in_place(accelerator, kinds):
         assert not any(bool(v.any()) for v in views)
 
 
+def test_some_views_in_place_and_some_not(accelerator):
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    views = _views(gen, [70_001, 40_000, 9, 8_200, 100], ["bf16", "fp32"], True)
+    before, out = [v.clone() for v in views], torch.zeros(1, device="cuda")
+    for max_norm in (1e9, 2.0):
+        outputs = [v if i % 2 else torch.full_like(v, 7.0, dtype=torch.float16) for i, v in enumerate(views)]
+        accelerator.CreateGradientClip()(None, views, outputs, max_norm, out, _temp(accelerator, views))
+        for v, b, o in zip(views, before, outputs):
+            assert_within(o, *clipped(b, float(out), max_norm, o.dtype))
+            assert v is o or torch.equal(v, b)
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 def test_a_norm_that_is_not_finite_changes_nothing(accelerator, bad):
     views = [torch.randn(9_000, device="cuda"), torch.randn(30, device="cuda").to(torch.bfloat16)]
