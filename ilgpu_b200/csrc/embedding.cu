@@ -11,11 +11,12 @@
 
 namespace b200alg {
 
-// Where rows do not lie on boundaries that groups can be moved from and to whole, groups of four columns begin on the
+// Where rows do not lie on boundaries that groups can be moved from and to whole, groups of four or eight columns begin on the
 // boundaries of the OUTPUT row (the first and the last one of a row stick out of it), and are put together from the two
 // aligned words of the input that hold them.  SHIFTED below.  (One element at a time: 60001 rows of 1357
-// bf16 184 us instead of 79.)
-constexpr int kShiftedGroup = 4;
+// bf16 184 us instead of 59.)
+constexpr int kMostShifted = 8;
+template <typename TIn, typename TOut> constexpr int shifted_group() { return sizeof(TIn) == 2 && sizeof(TOut) == 2 ? 8 : 4; }
 
 // Extent of a matrix that is read: a word that overlaps it may be loaded whole (an aligned word lies in one page).
 struct Extent {
@@ -32,7 +33,7 @@ template <typename T, int G, bool SHIFTED> struct Columns {  // G columns of a r
     __device__ __forceinline__ Group<T, G> get() const { return w; }
 };
 template <typename T, int G> struct Columns<T, G, true> {
-    static_assert(G == kShiftedGroup, "two words, of which four elements are chosen");
+    static_assert(G == 4 || (G == 8 && sizeof(T) == 2), "two words of 8 or 16 bytes, of which half the elements are chosen");
     Group<T, G> w, behind;
     int shift;  // elements of w in front of the first column
     __device__ __forceinline__ void load(const T *p, const Extent &matrix) {
@@ -50,19 +51,18 @@ template <typename T, int G> struct Columns<T, G, true> {
         shift = 0;
     }
     __device__ __forceinline__ Group<T, G> get() const {
+        constexpr int W = Group<T, G>::kWords, PER = 4 / (int)sizeof(T);  // elements of a word
+        unsigned int t[2 * W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = w.w[i], t[W + i] = behind.w[i];
+        const int words = shift / PER;  // by whole words, then by half a word
+#pragma unroll
+        for (int by = W / 2; by > 0; by >>= 1)
+#pragma unroll
+            for (int i = 0; i + by < 2 * W; ++i) t[i] = words & by ? t[i + by] : t[i];
         Group<T, G> r;
-        if constexpr (sizeof(T) == 4) {
-            unsigned int t[5];
-            const unsigned int all[8] = {w.w[0], w.w[1], w.w[2], w.w[3], behind.w[0], behind.w[1], behind.w[2], behind.w[3]};
 #pragma unroll
-            for (int i = 0; i < 5; ++i) t[i] = shift & 2 ? all[i + 2] : all[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r.w[i] = shift & 1 ? t[i + 1] : t[i];
-        } else {
-            const unsigned int a = shift & 2 ? w.w[1] : w.w[0], b = shift & 2 ? behind.w[0] : w.w[1], c = shift & 2 ? behind.w[1] : behind.w[0];
-            r.w[0] = __funnelshift_r(a, b, shift % 2 * 16);
-            r.w[1] = __funnelshift_r(b, c, shift % 2 * 16);
-        }
+        for (int i = 0; i < W; ++i) r.w[i] = sizeof(T) == 4 ? t[i] : __funnelshift_r(t[i], t[i + 1], shift % PER * 16);
         return r;
     }
 };
@@ -509,7 +509,7 @@ static int gradient_layout(int64_t rows, int64_t width, int64_t n, GradientLayou
     if (rows > INT32_MAX || width > INT32_MAX || n > INT32_MAX) return B200ALG_TOO_LARGE;
     L.tile = gradient_tile(n, width);
     L.tiles = ceil_div(n, L.tile);
-    L.share_stride = round_up(width + kShiftedGroup, 8) + 8;  // a shifted row has a group or two more
+    L.share_stride = round_up(width + kMostShifted, 8) + 8;  // a shifted row has a group or two more
     const int rc = b200alg_radix_sort_temp_bytes(B200ALG_U32, n, 4, &L.sort_bytes);  // its part lies first, and with it its status word
     if (rc != B200ALG_OK) return rc;
     L.off_keys = round_up(L.sort_bytes, 256);
@@ -603,7 +603,7 @@ extern "C" int b200alg_embedding(void *stream, const void *table, int64_t rows, 
             if (fits(G)) return run_lookup<TIn, TOut, G, false>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
             if constexpr (G == 16)
                 if (fits(8)) return run_lookup<TIn, TOut, 8, false>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
-            return run_lookup<TIn, TOut, kShiftedGroup, true>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
+            return run_lookup<TIn, TOut, shifted_group<TIn, TOut>(), true>(s, table, rows, width, row_stride, view, n, scale, out, out_stride);
         });
     });
 }
@@ -645,7 +645,7 @@ extern "C" int b200alg_embedding_gradient(void *stream, const void *tokens, int6
             constexpr int G = 16 / sizeof(TIn);
             if (groups_aligned(upstream, upstream_stride, n, width, ib, G) && groups_aligned(gradient, row_stride, rows, width, ob, G))
                 return run_gradient<TIn, TOut, G, false>(s, c, view, L, upstream, gradient, temp);
-            return run_gradient<TIn, TOut, kShiftedGroup, true>(s, c, view, L, upstream, gradient, temp);
+            return run_gradient<TIn, TOut, shifted_group<TIn, TOut>(), true>(s, c, view, L, upstream, gradient, temp);
         });
     });
 }
