@@ -92,12 +92,21 @@ inline int64_t groups_in(int64_t width, int group, bool shifted) { return shifte
 // 4096 bf16 out of 128000: groups of 16 bytes 127 us, of 32 bytes 114.6, four of those 116.)
 constexpr int kLookupThreads = 256, kLookupItems = 2;
 
+struct LookupCall {
+    int64_t rows, width, row_stride, out_stride;
+    Extent extent;      // of the table
+    IndexView tokens;
+    int64_t first;      // row of the output
+    unsigned int total; // groups
+    FastDivide groups;  // of a row
+    float scale;        // (of a double, rounded once)
+};
+
 template <typename TIn, typename TOut, int G, bool SHIFTED>
-__global__ void __launch_bounds__(kLookupThreads)
-lookup_kernel(const TIn *__restrict__ table, int64_t rows, int64_t width, int64_t row_stride, Extent extent, IndexView tokens, int64_t first,
-              TOut *__restrict__ out, int64_t out_stride, unsigned int total, FastDivide groups, float scale) {
+__global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupCall c, const TIn *__restrict__ table, TOut *__restrict__ out) {
     grid_dependency_release();
     grid_dependency_wait();
+    const FastDivide groups = c.groups;
     const unsigned int base = blockIdx.x * (kLookupThreads * kLookupItems) + threadIdx.x;
     Columns<TIn, G, SHIFTED> in[kLookupItems];
     TOut *to[kLookupItems];
@@ -106,12 +115,12 @@ lookup_kernel(const TIn *__restrict__ table, int64_t rows, int64_t width, int64_
     for (int u = 0; u < kLookupItems; ++u) {
         const unsigned int q = base + u * kLookupThreads;
         to[u] = nullptr;
-        if (q < total) {
+        if (q < c.total) {
             const unsigned int row = groups(q);
-            const int64_t token = tokens[first + row];
-            to[u] = out + (first + row) * out_stride;
+            const int64_t token = c.tokens[c.first + row];
+            to[u] = out + (c.first + row) * c.out_stride;
             column[u] = column_of<SHIFTED, G>(to[u], q - row * groups.d);
-            if (token >= 0 && token < rows) in[u].load(table + token * row_stride + column[u], extent);
+            if (token >= 0 && token < c.rows) in[u].load(table + token * c.row_stride + column[u], c.extent);
             else in[u].clear();
         }
     }
@@ -121,8 +130,8 @@ lookup_kernel(const TIn *__restrict__ table, int64_t rows, int64_t width, int64_
         const Group<TIn, G> g = in[u].get();
         float x[G];
 #pragma unroll
-        for (int k = 0; k < G; ++k) x[k] = g.get(k) * scale;
-        put_columns<SHIFTED>(to[u], column[u], width, x);
+        for (int k = 0; k < G; ++k) x[k] = g.get(k) * c.scale;
+        put_columns<SHIFTED>(to[u], column[u], c.width, x);
     }
 }
 
@@ -134,9 +143,10 @@ static int run_lookup(cudaStream_t s, const void *table, int64_t rows, int64_t w
     if (most < 1) return B200ALG_TOO_LARGE;
     for (int64_t first = 0; first < n; first += most) {
         const int64_t total = (n - first < most ? n - first : most) * groups;
+        const LookupCall c{rows, width, row_stride, out_stride, extent_of(table, rows, width, row_stride, sizeof(TIn)), tokens, first, (unsigned int)total,
+                           FastDivide((unsigned int)groups), (float)scale};
         B200ALG_CUDA_TRY(launch_dependent(lookup_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)ceil_div(total, kLookupThreads * kLookupItems)),
-                                          dim3(kLookupThreads), 0, s, (const TIn *)table, rows, width, row_stride,
-                                          extent_of(table, rows, width, row_stride, sizeof(TIn)), tokens, first, (TOut *)out, out_stride, (unsigned int)total, FastDivide((unsigned int)groups), (float)scale));
+                                          dim3(kLookupThreads), 0, s, c, (const TIn *)table, (TOut *)out));
     }
     return B200ALG_OK;
 }
