@@ -229,15 +229,13 @@ template <int G> __device__ __forceinline__ void write_share(float *p, const flo
     o.store(p);
 }
 
-// Clears those of the rows from `first` on, up to 32, whose bit in `rows` is set; by a warp.
-template <bool SHIFTED, int G, typename TOut> __device__ __forceinline__ void clear_rows(const GradientCall &c, TOut *out, int64_t first, unsigned int rows) {
+// Clears a row, by `threads` threads of which this is one.
+template <bool SHIFTED, int G, typename TOut> __device__ __forceinline__ void clear_row(const GradientCall &c, TOut *out, int64_t at, int thread, int threads) {
     float zero[G];
 #pragma unroll
     for (int k = 0; k < G; ++k) zero[k] = 0.0f;
-    for (; rows; rows &= rows - 1) {
-        TOut *row = out + (first + __ffs(rows) - 1) * c.row_stride;
-        for (int g = threadIdx.x & 31; g < c.groups; g += 32) put_columns<SHIFTED>(row, column_of<SHIFTED, G>(row, g), c.width, zero);
-    }
+    TOut *row = out + at * c.row_stride;
+    for (int g = thread; g < c.groups; g += threads) put_columns<SHIFTED>(row, column_of<SHIFTED, G>(row, g), c.width, zero);
 }
 
 template <typename TIn, typename TOut, int G, bool SHIFTED>
@@ -245,10 +243,12 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(Gradient
     grid_dependency_release();
     if (blockIdx.x < c.clear_blocks) {
         if (!c.early) grid_dependency_wait();
+        const int64_t first = (int64_t)blockIdx.x * c.clear_rows, behind = first + c.clear_rows < c.rows ? first + c.clear_rows : c.rows;
         const int lane = threadIdx.x & 31, each = c.clear_rows / (kGradientThreads / 32);  // rows of a warp
-        const int64_t begin = (int64_t)blockIdx.x * c.clear_rows + (threadIdx.x >> 5) * each, end = begin + each < c.rows ? begin + each : c.rows;
-        for (int64_t first = begin; first < end; first += 32)
-            clear_rows<SHIFTED, G>(c, out, first, __ballot_sync(0xffffffffu, first + lane < end && !c.named[first + lane]));
+        const int64_t begin = first + (threadIdx.x >> 5) * each, end = begin + each < behind ? begin + each : behind;
+        for (int64_t some = begin; some < end; some += 32)
+            for (unsigned int rows = __ballot_sync(0xffffffffu, some + lane < end && !c.named[some + lane]); rows; rows &= rows - 1)
+                clear_row<SHIFTED, G>(c, out, some + __ffs(rows) - 1, lane, 32);
         return;
     }
     grid_dependency_wait();
@@ -420,14 +420,14 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
 // lists the positions that name the row and adds them up, in y parts that are joined in order.  What clears does so with
 // the bits of its own rows, from all tokens as well.  (Sorting them would take one block 13 us and the launches around it
 // 5, whatever the table.)
-constexpr int64_t kFewTokens = 512;
+constexpr int64_t kFewTokens = 512, kMostFewTokens = 1024;  // the latter where a row is one part of a block: 840 of 64 floats 10 us, by a sort 19
 
 template <typename TIn, typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kGradientThreads)
 gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ upstream, TOut *__restrict__ out, TempHeader *hdr) {
     grid_dependency_release();
-    __shared__ unsigned int bits[kFewTokens / 32];
-    __shared__ unsigned short list[kFewTokens];
+    __shared__ unsigned int bits[kMostFewTokens / 32];
+    __shared__ unsigned short list[kMostFewTokens];
     __shared__ float part[kGradientThreads * G];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (int)c.n;
     // blocks that clear evenly between those that sum
@@ -443,23 +443,25 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
             if (token >= first && token < first + c.clear_rows) atomicOr(bits + ((token - first) >> 5), 1u << ((token - first) & 31));
         }
         __syncthreads();
-        for (int i = warp; i < c.clear_rows; i += kGradientThreads / 32)
-            if (first + i < c.rows && !(bits[i >> 5] >> (i & 31) & 1)) clear_rows<SHIFTED, G>(c, out, first + i, 1u);
+        const bool one_by_one = c.clear_rows < kGradientThreads / 32;  // long rows: all threads take one at a time
+        for (int i = one_by_one ? 0 : warp; i < c.clear_rows; i += one_by_one ? 1 : kGradientThreads / 32)
+            if (first + i < c.rows && !(bits[i >> 5] >> (i & 31) & 1))
+                clear_row<SHIFTED, G>(c, out, first + i, one_by_one ? threadIdx.x : lane, one_by_one ? kGradientThreads : 32);
         return;
     }
     grid_dependency_wait();
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) hdr->wait_limit_hit = 0u;
     const int i = (int)(block / c.slabs);
-    int64_t some[kFewTokens / kGradientThreads];  // this thread's share of the tokens, all under way at once
+    int64_t some[kMostFewTokens / kGradientThreads];  // this thread's share of the tokens, all under way at once
 #pragma unroll
-    for (int u = 0; u < kFewTokens / kGradientThreads; ++u) {
+    for (int u = 0; u < kMostFewTokens / kGradientThreads; ++u) {
         const int j = u * kGradientThreads + (int)threadIdx.x;
         some[u] = j < n ? tokens[j] : -1;
     }
     const int64_t token = tokens[i];
     if (token < 0 || token >= c.rows) return;
 #pragma unroll
-    for (int u = 0; u < kFewTokens / kGradientThreads; ++u) {
+    for (int u = 0; u < kMostFewTokens / kGradientThreads; ++u) {
         const unsigned int same = __ballot_sync(0xffffffffu, some[u] == token);
         if (lane == 0) bits[u * (kGradientThreads / 32) + warp] = same;
     }
@@ -531,10 +533,13 @@ static int gradient_layout(int64_t rows, int64_t width, int64_t n, GradientLayou
     return B200ALG_OK;
 }
 
-// Rows that a block clears: about 32 KB of them (64 and 128 KB: 9.5 and 15.9 instead of 8.5 us for 301 tokens into 10007 rows of 768 floats).
-static int rows_to_clear(int64_t width, int bytes, int most) {
-    const int64_t rows = (32 << 10) / (width * bytes);
-    return (int)(rows < kGradientThreads / 32 ? kGradientThreads / 32 : rows > most ? most : rows / (kGradientThreads / 32) * (kGradientThreads / 32));
+// Rows that a block clears: about 32 KB of them (64 and 128 KB: 9.5 and 15.9 instead of 8.5 us for 301 tokens into 10007
+// rows of 768 floats), but not fewer than `least`.  From a row for each warp on they are a multiple of that.
+static int rows_to_clear(int64_t width, int bytes, int least, int most) {
+    constexpr int kWarps = kGradientThreads / 32;
+    int64_t rows = (32 << 10) / (width * bytes);
+    rows = rows < least ? least : rows > most ? most : rows;
+    return (int)(rows < kWarps ? rows : rows / kWarps * kWarps);
 }
 
 template <typename TIn, typename TOut, int G, bool SHIFTED>
@@ -542,12 +547,12 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     c.groups = (int)groups_in(c.width, G, SHIFTED);
     c.extent = extent_of(upstream, c.n, c.width, c.upstream_stride, sizeof(TIn));
     char *t = (char *)temp;
-    if (c.n <= kFewTokens) {
+    if (c.n <= (c.groups <= kPartThreads ? kMostFewTokens : kFewTokens)) {
         // columns of a position that different blocks take: as many as make some thousands of blocks
         const int64_t slabs = ceil_div(c.groups, kPartThreads), most = ceil_div(2048, c.n ? c.n : 1);
         c.slabs = (int)(slabs < most ? slabs : most);
         c.sum_blocks = c.n * c.slabs;
-        c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 256);
+        c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 1, 256);
         c.clear_blocks = c.accumulate ? 0 : ceil_div(c.rows, c.clear_rows);
         const int64_t blocks = c.sum_blocks + c.clear_blocks;
         if (blocks > INT32_MAX) return B200ALG_TOO_LARGE;
@@ -565,7 +570,8 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     c.y = kGradientThreads / c.x;
     c.slabs = (int)ceil_div(c.groups, c.x);
     c.sum_blocks = ceil_div(c.tiles, c.y) * c.slabs;
-    c.clear_rows = rows_to_clear(c.width, sizeof(TOut), 1 << 20);
+    // (a row for each warp at least: with one row a block 131072 tokens of 4096 took 559 us instead of 528)
+    c.clear_rows = rows_to_clear(c.width, sizeof(TOut), kGradientThreads / 32, 1 << 20);
     c.clear_blocks = named ? ceil_div(c.rows, c.clear_rows) : 0;
     const int x = part_threads(c.groups);
     const int64_t join_blocks = ceil_div(c.tiles, kGradientThreads / x) * ceil_div(c.groups, x);

@@ -133,6 +133,7 @@ GRADIENT_SHAPES = [  # tokens, rows, width: one token, tiles of every length, ru
     (1, 1, 1), (1, 40, 8), (2, 3, 5), (15, 4, 64), (16, 100, 64), (17, 3, 33), (129, 9, 48), (300, 2000, 768), (2_367, 31, 40), (2_368, 5, 8),
     (4_737, 700, 129), (20_000, 37, 24), (19_001, 5000, 64), (500, 300, 4_100), (512, 90, 72), (513, 90, 72), (5_000, 30_000, 256), (60_000, 9, 16),
     (3_000, 50_000, 33), (10_000, 77, 2_051), (2_000_003, 5_000, 8),
+    (1_024, 300, 64), (1_025, 300, 64), (900, 40, 261), (90, 700, 9_001),
 ]
 
 
