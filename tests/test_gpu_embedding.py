@@ -231,6 +231,42 @@ def test_what_is_not_finite_stays_in_its_row_and_column(accelerator, n):
     assert int((~out.isfinite()).sum()) == 3
 
 
+@pytest.mark.parametrize("n", [300, 6_000, 60_000])
+def test_calls_in_a_row_over_the_same_buffers(accelerator, n):
+    """What clears rows starts while the sort runs: not before the kernel that reads the last call's result, or writes the
+    tokens, is through."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    rows, width = 20_000, 128
+    sets = [(torch.randint(0, rows, (n,), generator=gen, device="cuda"), torch.randn(n, width, generator=gen, device="cuda")) for _ in range(3)]
+    out, temp = torch.empty(rows, width, device="cuda"), accelerator.Allocate1D(accelerator.ComputeEmbeddingGradientTempStorageSize(rows, width, n), torch.int32)
+    call, want = accelerator.CreateEmbeddingGradient(), []
+    for tokens, upstream in sets:
+        call(None, tokens, upstream, out, temp)
+        torch.cuda.synchronize()
+        want.append(out.clone())
+        assert_within(out, *embedding_gradient(tokens, upstream, 1.0, rows, torch.float32))
+    tokens, seen = torch.empty_like(sets[0][0]), []
+    for i in range(12):
+        tokens.copy_(sets[i % 3][0])
+        call(None, tokens, sets[i % 3][1], out, temp)
+        seen.append(out * 1.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(3):
+            tokens.copy_(sets[i][0])
+            call(None, tokens, sets[i][1], out, temp)
+            seen[i].copy_(out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(s, want[i % 3]) for i, s in enumerate(seen))
+    for s in seen[:3]:
+        s.zero_()
+    for _ in range(4):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(s, w) for s, w in zip(seen, want))
+    del graph
+
+
 def test_gradient_is_the_lookups(accelerator):
     """Against differences: <lookup(table + d) - lookup(table), g> = <d, gradient(g)>, exactly linear."""
     gen = torch.Generator(device="cuda").manual_seed(6)

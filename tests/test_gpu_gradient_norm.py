@@ -152,6 +152,31 @@ def test_bits_do_not_change(accelerator):
     assert all(_norm(accelerator, views) == first for _ in range(5))
 
 
+@pytest.mark.parametrize("count", [3, 65, 257, 1_100])
+def test_captured_and_replayed(accelerator, count):
+    """The lists of all table sizes, and of two launches, are the graph's own."""
+    gen = torch.Generator(device="cuda").manual_seed(count)
+    views = _views(gen, [(i * 37) % 500 for i in range(count)], ["fp32", "bf16"], True)
+    results, out, temp = [torch.empty_like(v) for v in views], torch.zeros(1, device="cuda"), _temp(accelerator, views)
+    clip = accelerator.CreateGradientClip()
+    clip(None, views, results, 1.0, out, temp)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        clip(None, views, results, 1.0, out, temp)
+        clip(None, views, results, 1.0, out, temp)
+    for _ in range(3):
+        for v in views:
+            v.normal_(generator=gen)
+        graph.replay()
+        torch.cuda.synchronize()
+        whole = norm(views)
+        assert abs(float(out) - whole) <= NORM_BOUND * whole
+        for v, r in list(zip(views, results))[::17]:
+            assert_within(r, *clipped(v, float(out), 1.0, r.dtype))
+    del graph
+
+
 def test_a_view_past_32_bits_of_elements(accelerator):
     n = (1 << 32) + 77
     view = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
