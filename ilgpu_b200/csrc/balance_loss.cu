@@ -476,28 +476,54 @@ balance_gradient_kernel(BalanceCall call, const T *__restrict__ logits, const in
     }
 }
 
-// Calls `call` with the element type and the shape of a row.  A lane holds about 16 elements of a row where the row is
+// Elements of a group that a router's rows can be moved in: 16 bytes, or four, two or one element.
+static int router_group(int64_t experts, int bytes, const void *logits, int64_t logits_stride, const void *gradient, int64_t gradient_stride, int64_t tokens) {
+    auto fits = [&](int group) {
+        return groups_aligned(logits, logits_stride, tokens, experts, bytes, group) && groups_aligned(gradient, gradient_stride, tokens, experts, bytes, group);
+    };
+    const int most = 16 / bytes;
+    return fits(most) ? most : fits(4) ? 4 : fits(2) ? 2 : 1;
+}
+
+// Calls `call` with the element type and the shape of a row.  A lane holds 16 or 32 elements of a row where the row is
 // that long, so that few lanes share a row and few shuffles go into its maximum and its sum.
-template <typename Call> static int with_row(int dtype, int experts, bool whole_groups, Call call) {
+template <int V, typename T, typename Call> static int with_shape(int experts, Call call) {
+    const int groups = experts / V;
+    if constexpr (V >= 4) {
+        if (groups <= 2) return call(T{}, RowShape<V, 1, 2, 4>{});
+        if (groups <= 8) return call(T{}, RowShape<V, 2, 4, 2>{});
+        if (groups <= 16) return call(T{}, RowShape<V, 4, 4, 1>{});
+        if (groups <= 32) return call(T{}, RowShape<V, 4, 8, 1>{});
+        if (groups <= 64) return call(T{}, RowShape<V, 4, 16, 1>{});
+        if constexpr (V == 4) {
+            if (groups <= 128) return call(T{}, RowShape<V, 4, 32, 1>{});
+            return call(T{}, RowShape<V, 8, 32, 1>{});
+        } else {
+            return call(T{}, RowShape<V, 4, 32, 1>{});
+        }
+    } else {
+        constexpr int C = 8;
+        if constexpr (V == 2)  // (two lanes a row would read 16 bytes of it at a time)
+            if (groups <= 2 * C) return call(T{}, RowShape<V, 4, 4, 2>{});
+        if constexpr (V == 1)
+            if (groups <= 2 * C) return call(T{}, RowShape<V, C, 2, 2>{});
+        if (groups <= 4 * C) return call(T{}, RowShape<V, C, 4, 2 / V>{});
+        if (groups <= 8 * C) return call(T{}, RowShape<V, C, 8, 2 / V>{});
+        if constexpr (V == 1)
+            if (groups <= 12 * C) return call(T{}, RowShape<V, 12, 8, 1>{});
+        if (groups <= 16 * C) return call(T{}, RowShape<V, C, 16, 2 / V>{});
+        if (groups <= 32 * C) return call(T{}, RowShape<V, C, 32, 2 / V>{});
+        return call(T{}, RowShape<V, 32 / V, 32, 1>{});
+    }
+}
+template <typename Call> static int with_row(int dtype, int experts, int group, Call call) {
     return with_element(dtype, [&](auto element) {
         using T = decltype(element);
-        constexpr int V = 16 / sizeof(T), C = 4;
-        if (whole_groups) {
-            const int groups = experts / V;
-            if (groups <= 2) return call(element, RowShape<V, 1, 2, 4>{});
-            if (groups <= 8) return call(element, RowShape<V, 2, 4, 2>{});
-            if (groups <= 16) return call(element, RowShape<V, C, 4, 1>{});
-            if (groups <= 32) return call(element, RowShape<V, C, 8, 1>{});
-            if (groups <= 64) return call(element, RowShape<V, C, 16, 1>{});
-            if (groups <= 128) return call(element, RowShape<V, C, 32, 1>{});
-            if constexpr (V == 4) return call(element, RowShape<V, 2 * C, 32, 1>{});
-            return (int)B200ALG_UNSUPPORTED;  // (no type has more: 1024 experts are the most)
-        }
-        if (experts <= 16) return call(element, RowShape<1, 8, 2, 2>{});
-        if (experts <= 64) return call(element, RowShape<1, 8, 8, 2>{});
-        if (experts <= 128) return call(element, RowShape<1, 8, 16, 2>{});
-        if (experts <= 256) return call(element, RowShape<1, 8, 32, 2>{});
-        return call(element, RowShape<1, 32, 32, 1>{});
+        if (group == 1) return with_shape<1, T>(experts, call);
+        if (group == 2) return with_shape<2, T>(experts, call);
+        if constexpr (sizeof(T) == 2)
+            if (group == 8) return with_shape<8, T>(experts, call);
+        return with_shape<4, T>(experts, call);
     });
 }
 
@@ -508,9 +534,9 @@ template <typename S> static BalanceCall balance_call(int64_t tokens, int64_t lo
 // Blocks of a call: one for a few rows, then a cluster of them, and from where one is slower than two launches (0) as
 // many as there is work for.  In bf16 64 experts, us, cluster / two launches: 2048 tokens 6.6 / 7.2, 4096 8.9 / 7.6; rows
 // that do not lie on boundaries take longer: 1576 tokens of 99 experts in float 13.7 / 8.
-static int balance_cluster(int64_t tokens, int64_t experts, bool whole_groups) {
+static int balance_cluster(int64_t tokens, int64_t experts, bool long_groups) {
     const int64_t cells = tokens * experts;
-    return cells <= 4096 ? 1 : cells <= (whole_groups ? 1 << 17 : 1 << 15) ? kBalanceCluster : 0;
+    return cells <= 4096 ? 1 : cells <= (long_groups ? 1 << 17 : 1 << 15) ? kBalanceCluster : 0;
 }
 
 // Resident blocks of a kernel on the whole GPU (asked once per context; `cache` is the kernel's own).
@@ -570,10 +596,10 @@ extern "C" int b200alg_balance_loss(void *stream, const void *logits, int64_t to
     shares.sums = (float *)((char *)temp + sizeof(TempHeader));
     shares.counts = (unsigned int *)((char *)temp + sizeof(TempHeader) + round_up(kMostBalanceBlocks * experts * 4, 256));
     const BalanceResult to{coefficient * experts / choices, loss, counts, probabilities};
-    const bool whole = groups_aligned(logits, logits_stride, tokens, experts, bytes, 16 / bytes);
-    const int cluster = balance_cluster(tokens, experts, whole);
+    const int group = router_group(experts, bytes, logits, logits_stride, logits, logits_stride, tokens);
+    const int cluster = balance_cluster(tokens, experts, group >= 4);
     const size_t smem = (size_t)padded_bins((int)experts) * (1 + kBalanceWarps) * 4 + (cluster ? (size_t)ceil_div(experts, cluster) * 8 : 0);
-    rc = with_row(dtype, (int)experts, whole, [&](auto element, auto shape) -> int {
+    rc = with_row(dtype, (int)experts, group, [&](auto element, auto shape) -> int {
         using T = decltype(element);
         using S = decltype(shape);
         auto kernel = balance_kernel<T, S>;
@@ -609,9 +635,8 @@ extern "C" int b200alg_balance_loss_gradient(void *stream, const void *logits, i
     const int bytes = element_bytes(dtype);
     if ((uintptr_t)logits % bytes || (uintptr_t)gradient % bytes || (uintptr_t)counts % 4 || (uintptr_t)loss_gradient % 4) return B200ALG_MISALIGNED;
     cudaStream_t s = (cudaStream_t)stream;
-    const bool whole = groups_aligned(logits, logits_stride, tokens, experts, bytes, 16 / bytes) &&
-                       groups_aligned(gradient, gradient_stride, tokens, experts, bytes, 16 / bytes);
-    return with_row(dtype, (int)experts, whole, [&](auto element, auto shape) -> int {
+    const int group = router_group(experts, bytes, logits, logits_stride, gradient, gradient_stride, tokens);
+    return with_row(dtype, (int)experts, group, [&](auto element, auto shape) -> int {
         using T = decltype(element);
         using S = decltype(shape);
         auto kernel = balance_gradient_kernel<T, S>;
