@@ -179,6 +179,8 @@ struct GradientCall {
     int slabs;          // blocks along the columns
     int64_t sum_blocks;
     int clear_rows;     // rows of a block that clears
+    int flat;           // whether it clears them as one stretch: short rows one behind the other
+    FastDivide by_width;
     int64_t clear_blocks;
     int early;          // what clears need not wait for the launch before
 };
@@ -238,12 +240,34 @@ template <bool SHIFTED, int G, typename TOut> __device__ __forceinline__ void cl
     for (int g = thread; g < c.groups; g += threads) put_columns<SHIFTED>(row, column_of<SHIFTED, G>(row, g), c.width, zero);
 }
 
+// Clears those of the `rows` rows from `first` on, one behind the other in memory, that are not named, word by word of 16
+// bytes whatever the rows' width; by a block.  (822 tokens into 60092 rows of 115 bf16: 10.6 us, row by row 22.7.)
+template <typename TOut, typename Named> __device__ __forceinline__ void clear_flat(const GradientCall &c, TOut *out, int64_t first, int rows, Named named) {
+    constexpr int W = 16 / (int)sizeof(TOut);
+    TOut *const base = out + first * c.width;
+    const int count = rows * (int)c.width, before = (int)((uintptr_t)base / sizeof(TOut) % W), words = (count + before + W - 1) / W;
+    for (int w = threadIdx.x; w < words; w += kGradientThreads) {
+        const int begin = w * W - before, from = begin < 0 ? 0 : begin, to = begin + W < count ? begin + W : count;
+        const int row = (int)c.by_width(from), last = (int)c.by_width(to - 1);
+        if (to - from == W && last - row <= 1 && !named(row) && !named(last)) {
+            *reinterpret_cast<uint4 *>(base + begin) = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            for (int e = from; e < to; ++e)
+                if (!named((int)c.by_width(e))) base[e] = from_float<TOut>(0.0f);
+        }
+    }
+}
+
 template <typename TIn, typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(GradientCall c, const TIn *__restrict__ upstream, TOut *__restrict__ out) {
     grid_dependency_release();
     if (blockIdx.x < c.clear_blocks) {
         if (!c.early) grid_dependency_wait();
         const int64_t first = (int64_t)blockIdx.x * c.clear_rows, behind = first + c.clear_rows < c.rows ? first + c.clear_rows : c.rows;
+        if (c.flat) {
+            clear_flat(c, out, first, (int)(behind - first), [&](int row) { return c.named[first + row] != 0; });
+            return;
+        }
         const int lane = threadIdx.x & 31, each = c.clear_rows / (kGradientThreads / 32);  // rows of a warp
         const int64_t begin = first + (threadIdx.x >> 5) * each, end = begin + each < behind ? begin + each : behind;
         for (int64_t some = begin; some < end; some += 32)
@@ -443,6 +467,11 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
             if (token >= first && token < first + c.clear_rows) atomicOr(bits + ((token - first) >> 5), 1u << ((token - first) & 31));
         }
         __syncthreads();
+        if (c.flat) {
+            clear_flat(c, out, first, (int)(first + c.clear_rows < c.rows ? c.clear_rows : c.rows - first),
+                       [&](int row) { return (bits[row >> 5] >> (row & 31) & 1) != 0; });
+            return;
+        }
         const bool one_by_one = c.clear_rows < kGradientThreads / 32;  // long rows: all threads take one at a time
         for (int i = one_by_one ? 0 : warp; i < c.clear_rows; i += one_by_one ? 1 : kGradientThreads / 32)
             if (first + i < c.rows && !(bits[i >> 5] >> (i & 31) & 1))
@@ -547,6 +576,8 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     c.groups = (int)groups_in(c.width, G, SHIFTED);
     c.extent = extent_of(upstream, c.n, c.width, c.upstream_stride, sizeof(TIn));
     char *t = (char *)temp;
+    c.flat = (c.row_stride == c.width || c.rows == 1) && c.width * (int64_t)sizeof(TOut) < 1024;  // (rows of 5 KB: 89 us instead of 80)
+    c.by_width = FastDivide((unsigned int)c.width);
     if (c.n <= (c.groups <= kPartThreads ? kMostFewTokens : kFewTokens)) {
         // columns of a position that different blocks take: as many as make some thousands of blocks
         const int64_t slabs = ceil_div(c.groups, kPartThreads), most = ceil_div(2048, c.n ? c.n : 1);
