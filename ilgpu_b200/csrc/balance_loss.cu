@@ -41,7 +41,10 @@ struct BalanceCall {
 
 __host__ __device__ constexpr int padded_bins(int experts) { return (experts + 4) / 4 * 4; }
 constexpr int kGradientWarps = 8;
-constexpr size_t kBalanceSmem = (size_t)padded_bins(kMostExperts) * (2 + kBalanceWarps) * 4;  // of balance_kernel at most
+// Shared memory of balance_kernel: counts, the warps' sums, and where one cluster is all a block's part of what it adds up.
+static size_t balance_smem(int64_t experts, int cluster) {
+    return (size_t)padded_bins((int)experts) * (1 + kBalanceWarps) * 4 + (cluster ? (size_t)ceil_div(experts, cluster) * 8 : 0);
+}
 
 __device__ __forceinline__ float exp2_approximate(float x) {  // 2^x; below 2^-126 zero
     float y;
@@ -598,13 +601,13 @@ extern "C" int b200alg_balance_loss(void *stream, const void *logits, int64_t to
     const BalanceResult to{coefficient * experts / choices, loss, counts, probabilities};
     const int group = router_group(experts, bytes, logits, logits_stride, logits, logits_stride, tokens);
     const int cluster = balance_cluster(tokens, experts, group >= 4);
-    const size_t smem = (size_t)padded_bins((int)experts) * (1 + kBalanceWarps) * 4 + (cluster ? (size_t)ceil_div(experts, cluster) * 8 : 0);
+    const size_t smem = balance_smem(experts, cluster);
     rc = with_row(dtype, (int)experts, group, [&](auto element, auto shape) -> int {
         using T = decltype(element);
         using S = decltype(shape);
         auto kernel = balance_kernel<T, S>;
         static ContextCache<int> cache;
-        const int status = resident_blocks(kernel, kBalanceThreads, kBalanceSmem, cache, &blocks);
+        const int status = resident_blocks(kernel, kBalanceThreads, balance_smem(kMostExperts, 1), cache, &blocks);
         if (status != B200ALG_OK) return status;
         if (cluster) {
             blocks = cluster;

@@ -48,7 +48,7 @@ def _router(gen, tokens, experts, choices, kind, ids, spread=2.0):
     (1, 1, 1), (1, 8, 2), (2, 3, 1), (31, 4, 4), (64, 8, 2), (65, 16, 3), (100, 24, 2), (1_000, 60, 4), (515, 61, 5), (2_000, 64, 8), (777, 128, 1), (130, 130, 2),
     (3_001, 160, 6), (500, 256, 8), (129, 257, 8), (70, 320, 2), (90, 512, 4), (40, 513, 3), (33, 768, 8), (20, 1_000, 2), (50, 1_023, 16), (48, 1_024, 1),
     (500, 21, 2), (501, 30, 3), (300, 38, 4), (301, 44, 2), (302, 62, 6), (200, 70, 2), (201, 93, 4), (150, 101, 2), (151, 122, 8), (70, 252, 2), (71, 258, 2), (60, 514, 2),
-    (40, 1_018, 3), (41, 1_012, 3)])
+    (40, 1_018, 3), (41, 1_012, 3), (1, 1_024, 2), (4, 1_024, 8), (3, 1_023, 2), (4, 1_000, 1)])
 def test_loss_and_gradient(accelerator, tokens, experts, choices, kind):
     gen = torch.Generator(device="cuda").manual_seed(tokens + experts)
     logits, chosen = _router(gen, tokens, experts, choices, kind, torch.int64 if tokens % 2 else torch.int32)
