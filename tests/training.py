@@ -99,7 +99,11 @@ class Balance:
         return value, bound + 2 * U * value.abs(), mean, off + U * mean
 
     def gradient(self, upstream, dtype, counts=None, number=None, base=None):
-        """The gradient and its bound, from counts of this call's own or given ones."""
+        """The gradient and its bound, from counts of this call's own or given ones.
+
+        An exp below 2^-126 that is taken as zero takes up to c 2^-126 from the row's sum of c p (1 / sum of exp <= 1), which p and the
+        factor multiply: factor p 2^-126 sum c in all.  Each of the two products may end below 2^-126, where half a step is 2^-150; the
+        second multiplies the first one's by |factor| at most."""
         c = (self.counts if counts is None else counts.cpu()[:self.experts]).double()
         number = self.number if number is None else number
         factor = upstream * self.coefficient * self.experts / self.choices / number ** 2 if number else 0.0
@@ -108,6 +112,7 @@ class Balance:
         row = self.relative.amax(dim=1, keepdim=True)
         off_dot = (2 * row + (self.experts + 6) * U) * dot
         bound = abs(factor) * self.p * ((self.relative + 6 * U) * (c - dot).abs() + off_dot + 2 * U * c) + 2.0 ** -120 * abs(factor) * (c + dot)
+        bound = bound + 2.0 ** -126 * abs(factor) * self.p * c.sum() + 2.0 ** -150 * (1.0 + abs(factor))
         exact, bound = torch.where(self.valid[:, None], exact, 0.0), torch.where(self.valid[:, None], bound, 0.0)
         if base is not None:
             exact = exact + base.cpu().double()
