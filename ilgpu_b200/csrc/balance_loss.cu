@@ -422,11 +422,18 @@ balance_gradient_kernel(BalanceCall call, const T *__restrict__ logits, const in
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lane_of_row = lane & (S::LANES - 1), row_of_warp = lane / S::LANES;
     const unsigned int rows = (unsigned int)call.tokens, apart = gridDim.x * (kGradientWarps * S::ROWS);
-    Pair often[S::E / 2];
-    auto often_of = [&](int i) {  // of the lane's i-th element
+    // Counts from the smallest one on: what all experts share takes no part in c - dot, and left in it would round it.
+    // Where all are chosen as often the gradient is zero.
+    int number[S::E], least = INT32_MAX;
+#pragma unroll
+    for (int i = 0; i < S::E; ++i) {
         const int g = i / S::V * S::LANES + lane_of_row;
-        return g < call.groups ? (float)counts[g * S::V + i % S::V] : 0.0f;
-    };
+        number[i] = g < call.groups ? counts[g * S::V + i % S::V] : INT32_MAX;  // of the lane's i-th element
+        least = min(least, number[i]);
+    }
+    least = __reduce_min_sync(0xFFFFFFFFu, least);
+    auto often_of = [&](int i) { return i / S::V * S::LANES + lane_of_row < call.groups ? (float)((unsigned int)number[i] - (unsigned int)least) : 0.0f; };
+    Pair often[S::E / 2];
 #pragma unroll
     for (int i = 0; i < S::E / 2; ++i) often[i] = Pair(often_of(2 * i), often_of(2 * i + 1));
     const double tokens = counts[call.experts];

@@ -153,6 +153,19 @@ def test_gradient_against_differences(accelerator):
         assert abs((up - down) / (2 * h) - slope) <= h * h * 12 * float(d.abs().max()) ** 3 + 1e-11 + 1e-5 * float((gradient.double() * d).abs().sum())
 
 
+@pytest.mark.parametrize("tokens, experts, stride", [(1, 1, 1), (300, 8, 8), (123, 60, 60), (77, 61, 64), (40, 300, 301), (9, 1_024, 1_024)])
+def test_experts_chosen_alike(accelerator, tokens, experts, stride):
+    """Where every expert is chosen as often, nothing is to be learnt: the gradient is zero, not what rounding leaves of it."""
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    logits = torch.randn(tokens, stride, generator=gen, device="cuda")[:, :experts]
+    chosen = torch.arange(experts, device="cuda").expand(tokens, experts).contiguous()
+    _, counts, _ = _run(accelerator, logits, chosen)
+    assert counts.tolist() == [tokens] * (experts + 1)
+    gradient = torch.full((tokens, experts), math.nan, device="cuda")
+    accelerator.CreateBalanceLossGradient(1.0, experts)(None, logits, None, counts, torch.full((1,), 1e6, device="cuda"), gradient)
+    assert not bool(gradient.any())
+
+
 def test_counts_of_all_ranks(accelerator):
     """Counts and tokens that were summed over ranks."""
     gen = torch.Generator(device="cuda").manual_seed(9)
