@@ -157,9 +157,11 @@ static int run_lookup(cudaStream_t s, const void *table, int64_t rows, int64_t w
 // positions is summed by the threads of a block, each holding one group of columns in registers and walking along the
 // tile.  A run of equal tokens inside a tile is written at once; a tile's share of a run that crosses its border goes to
 // temp, and gradient_join_kernel adds the shares up in order.  Rows that no token names, which are most of a large
-// table, are cleared by the other blocks of the same launch.  They know them from a byte per row and need not wait for the
-// sort, so that its time passes behind them.  Memory is the bound: 131072 rows of 4096 bf16 into 128000 rows of float take
-// 518 us, 3.2 GB at 6.0 TB/s; 16384 of 2048 into 32000 take 67, 55 of them in this kernel at 6.0 TB/s.
+// table, are known from a byte each and cleared by other blocks of the last launch, beside the join, which waits more than it
+// moves.  (Beside the sums the join stands alone at the end: 75.8 us instead of 70.3 for 16384 tokens.  The sort, too, is
+// independent of the clearing, but a launch that passes it by without a wait is not promised to find the bytes written.)
+// Memory is the bound: 131072 rows of 4096 bf16 into 128000 rows of float take 526 us, 3.2 GB at 5.9 TB/s; 16384 of 2048
+// into 32000 take 70, some 15 of them for keys and sort in front of 330 MB.
 constexpr int kGradientThreads = 256;
 constexpr int kAhead = 8;      // rows, or shares, that a thread has in flight
 
@@ -181,8 +183,7 @@ struct GradientCall {
     int clear_rows;     // rows of a block that clears
     int flat;           // whether it clears them as one stretch: short rows one behind the other
     FastDivide by_width;
-    int64_t clear_blocks;
-    int early;          // what clears need not wait for the launch before
+    int64_t clear_blocks, join_blocks;
 };
 
 __global__ void __launch_bounds__(256) gradient_forget_kernel(uint4 *named, int64_t words) {
@@ -261,22 +262,8 @@ template <typename TOut, typename Named> __device__ __forceinline__ void clear_f
 template <typename TIn, typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kGradientThreads) gradient_sum_kernel(GradientCall c, const TIn *__restrict__ upstream, TOut *__restrict__ out) {
     grid_dependency_release();
-    if (blockIdx.x < c.clear_blocks) {
-        if (!c.early) grid_dependency_wait();
-        const int64_t first = (int64_t)blockIdx.x * c.clear_rows, behind = first + c.clear_rows < c.rows ? first + c.clear_rows : c.rows;
-        if (c.flat) {
-            clear_flat(c, out, first, (int)(behind - first), [&](int row) { return c.named[first + row] != 0; });
-            return;
-        }
-        const int lane = threadIdx.x & 31, each = c.clear_rows / (kGradientThreads / 32);  // rows of a warp
-        const int64_t begin = first + (threadIdx.x >> 5) * each, end = begin + each < behind ? begin + each : behind;
-        for (int64_t some = begin; some < end; some += 32)
-            for (unsigned int rows = __ballot_sync(0xffffffffu, some + lane < end && !c.named[some + lane]); rows; rows &= rows - 1)
-                clear_row<SHIFTED, G>(c, out, some + __ffs(rows) - 1, lane, 32);
-        return;
-    }
     grid_dependency_wait();
-    const unsigned int rows = (unsigned int)c.rows, block = blockIdx.x - (unsigned int)c.clear_blocks;
+    const unsigned int rows = (unsigned int)c.rows, block = blockIdx.x;
     const int tx = threadIdx.x % c.x, ty = threadIdx.x / c.x;
     const int64_t t = (int64_t)(block / c.slabs) * c.y + ty;
     const int g = (int)(block % c.slabs) * c.x + tx;
@@ -378,6 +365,20 @@ __device__ __forceinline__ void add_shares(float (&sum)[G], const GradientCall &
     }
 }
 
+// Clears those of a block's rows that no token names.
+template <bool SHIFTED, int G, typename TOut> __device__ __forceinline__ void clear_unnamed(const GradientCall &c, TOut *out, int64_t block) {
+    const int64_t first = block * c.clear_rows, behind = first + c.clear_rows < c.rows ? first + c.clear_rows : c.rows;
+    if (c.flat) {
+        clear_flat(c, out, first, (int)(behind - first), [&](int row) { return c.named[first + row] != 0; });
+        return;
+    }
+    const int lane = threadIdx.x & 31, each = c.clear_rows / (kGradientThreads / 32);  // rows of a warp
+    const int64_t begin = first + (threadIdx.x >> 5) * each, end = begin + each < behind ? begin + each : behind;
+    for (int64_t some = begin; some < end; some += 32)
+        for (unsigned int rows = __ballot_sync(0xffffffffu, some + lane < end && !c.named[some + lane]); rows; rows &= rows - 1)
+            clear_row<SHIFTED, G>(c, out, some + __ffs(rows) - 1, lane, 32);
+}
+
 template <typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(GradientCall c, TOut *__restrict__ out, int x) {
     __shared__ float part[kGradientThreads * G];
@@ -385,6 +386,10 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
     __shared__ unsigned int keys[kMostParts];
     grid_dependency_release();
     grid_dependency_wait();
+    if (blockIdx.x >= c.join_blocks) {
+        clear_unnamed<SHIFTED, G>(c, out, blockIdx.x - c.join_blocks);
+        return;
+    }
     const int tx = threadIdx.x & (x - 1), ty = threadIdx.x / x, parts = kGradientThreads / x, lane = threadIdx.x & 31;
     const int slabs = (c.groups + x - 1) / x, g = (int)(blockIdx.x % slabs) * x + tx;
     const int64_t first = (int64_t)(blockIdx.x / slabs) * parts;
@@ -605,21 +610,19 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     c.clear_rows = rows_to_clear(c.width, sizeof(TOut), kGradientThreads / 32, 1 << 20);
     c.clear_blocks = named ? ceil_div(c.rows, c.clear_rows) : 0;
     const int x = part_threads(c.groups);
-    const int64_t join_blocks = ceil_div(c.tiles, kGradientThreads / x) * ceil_div(c.groups, x);
-    if (c.sum_blocks + c.clear_blocks > INT32_MAX || join_blocks > INT32_MAX) return B200ALG_TOO_LARGE;
+    c.join_blocks = ceil_div(c.tiles, kGradientThreads / x) * ceil_div(c.groups, x);
+    if (c.sum_blocks > INT32_MAX || c.join_blocks + c.clear_blocks > INT32_MAX) return B200ALG_TOO_LARGE;
     const int64_t cap = (int64_t)sm_count() * 8;
     auto some = [&](int64_t want) { return dim3((unsigned)(want < cap ? want : cap)); };
     if (named)
         B200ALG_CUDA_TRY(launch_dependent(gradient_forget_kernel, some(ceil_div(L.named_words, 256)), dim3(256), 0, s, (uint4 *)named, L.named_words));
     B200ALG_CUDA_TRY(launch_dependent(gradient_keys_kernel, some(ceil_div(c.n, 256 * 2)), dim3(256), 0, s, tokens, c.n, c.rows, keys, named));
-    bool one_launch = false;
-    const int rc = sort_with_positions(s, keys, positions, c.n, temp, L.sort_bytes, &one_launch);
+    const int rc = sort_with_positions(s, keys, positions, c.n, temp, L.sort_bytes);
     if (rc != B200ALG_OK) return rc;
-    c.early = one_launch;
     const size_t smem = (size_t)c.y * (2 * c.tile + 3) * 4;  // (33 KB at most)
-    B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)(c.sum_blocks + c.clear_blocks)), dim3(kGradientThreads), smem, s, c,
+    B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)c.sum_blocks), dim3(kGradientThreads), smem, s, c,
                                       (const TIn *)upstream, (TOut *)out));
-    B200ALG_CUDA_TRY(launch_dependent(gradient_join_kernel<TOut, G, SHIFTED>, dim3((unsigned)join_blocks), dim3(kGradientThreads), 0, s, c, (TOut *)out, x));
+    B200ALG_CUDA_TRY(launch_dependent(gradient_join_kernel<TOut, G, SHIFTED>, dim3((unsigned)(c.join_blocks + c.clear_blocks)), dim3(kGradientThreads), 0, s, c, (TOut *)out, x));
     return B200ALG_OK;
 }
 

@@ -1344,10 +1344,8 @@ static int partition_key(cudaStream_t s, int kb, const void *keys, const void *v
     return B200ALG_UNSUPPORTED;
 }
 
-// *one_launch: whether the sort was one launch.
 static int sort_common(void *stream, const SortCall &call, int key_dtype, int value_bytes, int order, void *temp,
-                       int64_t temp_bytes, bool *one_launch = nullptr) {
-    if (one_launch) *one_launch = false;
+                       int64_t temp_bytes) {
     // Argument checks mirror VerifyArguments (RadixSortExtensions.cs:1340-1367).
     if (!call.in_keys || !call.out_keys || !temp || (value_bytes && !call.out_values)) return B200ALG_INVALID_ARGUMENT;
     if (value_bytes && !call.in_values && call.value_seq == kSeqNone) return B200ALG_INVALID_ARGUMENT;
@@ -1372,13 +1370,10 @@ static int sort_common(void *stream, const SortCall &call, int key_dtype, int va
         bool taken = false;
         const SortScratch scratch{(char *)temp + L.off_keys, (char *)temp + L.off_values, L.control_bytes};
         int rc = block_sort(s, call, kb, value_bytes, xn, xp, temp, &taken);
-        if (one_launch) *one_launch = taken;
         if (rc != B200ALG_OK || taken) return rc;
         rc = sample_sort(s, call, kb, value_bytes, xn, xp, temp, scratch, &taken);
-        if (one_launch) *one_launch = taken;
         if (rc != B200ALG_OK || taken) return rc;
         rc = resident_sort(s, call, kb, value_bytes, xn, xp, temp, temp_bytes, &taken);
-        if (one_launch) *one_launch = taken;
         if (rc != B200ALG_OK || taken) return rc;
     }
     switch (value_bytes) {
@@ -1392,9 +1387,9 @@ static int sort_common(void *stream, const SortCall &call, int key_dtype, int va
     return B200ALG_UNSUPPORTED;
 }
 
-int sort_with_positions(void *stream, unsigned int *keys, unsigned int *positions, int64_t n, void *temp, int64_t temp_bytes, bool *one_launch) {
+int sort_with_positions(void *stream, unsigned int *keys, unsigned int *positions, int64_t n, void *temp, int64_t temp_bytes) {
     const SortCall call{keys, keys, positions, positions, 1, n, nullptr, kSeqInteger, false};
-    return sort_common(stream, call, B200ALG_U32, 4, B200ALG_SORT_ASCENDING, temp, temp_bytes, one_launch);
+    return sort_common(stream, call, B200ALG_U32, 4, B200ALG_SORT_ASCENDING, temp, temp_bytes);
 }
 
 }  // namespace b200alg
