@@ -538,12 +538,26 @@ gradient_few_kernel(GradientCall c, IndexView tokens, const TIn *__restrict__ up
     }
 }
 
+// Floats of a tile's share of a run (a shifted row has a group or two more than its columns).
+static int64_t share_floats(int64_t width) { return round_up(width + kMostShifted, 8) + 8; }
+
 // Sorted positions of a tile: enough blocks for the GPU (a narrow row leaves room for many tiles in one), and shares of
 // crossing runs that stay a small part of the traffic.
-static int64_t gradient_tile(int64_t n, int64_t width) {
-    int64_t tile = 128;
-    while (tile > 16 && ceil_div(n, tile) * (width < 2048 ? width : 2048) < (int64_t)148 * 3 / 2 * 2048) tile /= 2;
+constexpr int64_t kLeastTile = 16, kMostTile = 128;
+constexpr int64_t kEnoughTiles = 148 * 3 / 2, kWideShare = 2064;  // tiles of wide rows, from 2048 columns on
+static int64_t gradient_tile(int64_t n, int64_t share) {
+    int64_t tile = kMostTile;
+    while (tile > kLeastTile && ceil_div(n, tile) * (share < kWideShare ? share : kWideShare) < kEnoughTiles * kWideShare) tile /= 2;
     return tile;
+}
+// Floats that the shares of this many positions, or of fewer of no wider rows, take at most, so that a temp for the
+// longest input serves all.  A tile below the longest is half of one that was too long: kEnoughTiles wide shares were
+// more than all its shares, and those of its halves are at most twice as many.
+static int64_t most_share_floats(int64_t n, int64_t share) {
+    const int64_t longest = ceil_div(n, kMostTile) * share, least = ceil_div(n, kLeastTile) * share;
+    const int64_t halves = 2 * kEnoughTiles * (share > kWideShare ? share : kWideShare);
+    const int64_t shorter = least < halves ? least : halves;
+    return longest > shorter ? longest : shorter;
 }
 
 struct GradientLayout {
@@ -553,9 +567,9 @@ struct GradientLayout {
 static int gradient_layout(int64_t rows, int64_t width, int64_t n, GradientLayout &L) {
     if (rows < 0 || width < 0 || n < 0) return B200ALG_INVALID_ARGUMENT;
     if (rows > INT32_MAX || width > INT32_MAX || n > INT32_MAX) return B200ALG_TOO_LARGE;
-    L.tile = gradient_tile(n, width);
+    L.share_stride = share_floats(width);
+    L.tile = gradient_tile(n, L.share_stride);
     L.tiles = ceil_div(n, L.tile);
-    L.share_stride = round_up(width + kMostShifted, 8) + 8;  // a shifted row has a group or two more
     const int rc = b200alg_radix_sort_temp_bytes(B200ALG_U32, n, 4, &L.sort_bytes);  // its part lies first, and with it its status word
     if (rc != B200ALG_OK) return rc;
     L.off_keys = round_up(L.sort_bytes, 256);
@@ -563,7 +577,7 @@ static int gradient_layout(int64_t rows, int64_t width, int64_t n, GradientLayou
     L.off_named = L.off_positions + round_up(n * 4, 256);
     L.named_words = ceil_div(rows, 16);  // of 16 bytes
     L.off_shares = L.off_named + round_up(L.named_words * 16, 256);
-    L.total = L.off_shares + round_up(2 * L.tiles * L.share_stride * 4, 256);
+    L.total = L.off_shares + round_up(2 * most_share_floats(n, L.share_stride) * 4, 256);
     return B200ALG_OK;
 }
 

@@ -261,7 +261,8 @@ int b200alg_embedding(void *stream, const void *table, int64_t rows, int64_t wid
  * over all i with tokens[i] == v, in the order of i; every row of the table's gradient is
  * written, rows that no token names with zeros.  With accumulate != 0 the sums are added to
  * what `gradient` holds, and rows that no token names are left alone.  Tokens outside
- * [0, rows) add to nothing.  b200alg_device_status(temp) holds for this call. */
+ * [0, rows) add to nothing.  b200alg_device_status(temp) holds for this call.  A temp for the
+ * most rows, columns and tokens serves calls of fewer. */
 int b200alg_embedding_gradient_temp_bytes(int64_t rows, int64_t width, int64_t n, int64_t *out_bytes);
 int b200alg_embedding_gradient(void *stream, const void *tokens, int64_t n, int64_t token_stride, int token_dtype,
                                const void *upstream, int64_t upstream_stride, int upstream_dtype, double scale,

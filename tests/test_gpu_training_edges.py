@@ -1,0 +1,41 @@
+"""Calls at the edges of what the operators of a training step document: temps of other sizes, empty calls, values at the ends of
+their ranges."""
+import pytest
+import torch
+
+import ilgpu_b200 as ib
+
+from .training import TYPES, assert_within, embedding_gradient
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_temp_for_the_longest_batch_serves_the_shorter_ones(accelerator):
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    rows, width, most = 900, 512, 33_000
+    upstream = torch.randn(most, width, generator=gen, device="cuda").to(torch.bfloat16)
+    temp = accelerator.Allocate1D(accelerator.ComputeEmbeddingGradientTempStorageSize(rows, width, most), torch.int32)
+    call = accelerator.CreateEmbeddingGradient()
+    for n in (33_000, 28_288, 28_289, 16_384, 14_144, 8_192, 7_073, 7_000, 1_025, 600, 1, 0):
+        tokens = (torch.rand(n, generator=gen, device="cuda") ** 3 * rows).long()
+        for narrow in (width, 40):
+            temp.fill_(-1)
+            out = torch.full((rows, narrow), float("nan"), device="cuda")
+            call(None, tokens, upstream[:, :narrow], out, temp)
+            accelerator.CheckDeviceStatus(None, temp)
+            assert_within(out, *embedding_gradient(tokens, upstream[:, :narrow], 1.0, rows, torch.float32))
+
+
+@pytest.mark.parametrize("types", ["bf16 fp32", "fp32 fp32", "bf16 bf16"])
+@pytest.mark.parametrize("n, width", [(1_025, 1), (3_000, 33), (7_104, 2_051), (14_208, 512), (60_000, 9), (120_000, 64)])
+def test_nothing_is_written_behind_the_temp(accelerator, n, width, types):
+    """Every row crosses tiles, so that all shares are written."""
+    source, target = (TYPES[t] for t in types.split())
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    ints = accelerator.ComputeEmbeddingGradientTempStorageSize(3, width, n)
+    whole = torch.full((ints + 4_096,), 0x5A5A5A5A, dtype=torch.int32, device="cuda")
+    tokens = torch.randint(0, 3, (n,), generator=gen, device="cuda")
+    upstream, out = torch.randn(n, width, generator=gen, device="cuda").to(source), torch.empty(3, width, dtype=target, device="cuda")
+    accelerator.CreateEmbeddingGradient()(None, tokens, upstream, out, whole[:ints])
+    assert_within(out, *embedding_gradient(tokens, upstream, 1.0, 3, target))
+    assert bool((whole[ints:] == 0x5A5A5A5A).all())
