@@ -590,6 +590,12 @@ static int rows_to_clear(int64_t width, int bytes, int least, int most) {
     return (int)(rows < kWarps ? rows : rows / kWarps * kWarps);
 }
 
+// The status word of a call that has nothing else to do.
+static int clear_status(cudaStream_t s, void *temp) {
+    B200ALG_CUDA_TRY(cudaMemsetAsync(&((TempHeader *)temp)->wait_limit_hit, 0, sizeof(unsigned int), s));
+    return B200ALG_OK;
+}
+
 template <typename TIn, typename TOut, int G, bool SHIFTED>
 static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens, const GradientLayout &L, const void *upstream, void *out, void *temp) {
     c.groups = (int)groups_in(c.width, G, SHIFTED);
@@ -606,9 +612,9 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
         c.clear_blocks = c.accumulate ? 0 : ceil_div(c.rows, c.clear_rows);
         const int64_t blocks = c.sum_blocks + c.clear_blocks;
         if (blocks > INT32_MAX) return B200ALG_TOO_LARGE;
-        if (blocks)
-            B200ALG_CUDA_TRY(launch_dependent(gradient_few_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)blocks), dim3(kGradientThreads), 0, s, c, tokens,
-                                              (const TIn *)upstream, (TOut *)out, (TempHeader *)temp));
+        if (!blocks) return clear_status(s, temp);
+        B200ALG_CUDA_TRY(launch_dependent(gradient_few_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)blocks), dim3(kGradientThreads), 0, s, c, tokens,
+                                          (const TIn *)upstream, (TOut *)out, (TempHeader *)temp));
         return B200ALG_OK;
     }
     unsigned int *keys = (unsigned int *)(t + L.off_keys), *positions = (unsigned int *)(t + L.off_positions);
@@ -690,7 +696,7 @@ extern "C" int b200alg_embedding_gradient(void *stream, const void *tokens, int6
     GradientLayout L;
     int rc = gradient_layout(rows, width, n, L);
     if (rc != B200ALG_OK) return rc;
-    if (rows == 0 || width == 0) return B200ALG_OK;
+    if (rows == 0 || width == 0) return temp && temp_bytes >= (int64_t)sizeof(TempHeader) ? clear_status((cudaStream_t)stream, temp) : B200ALG_OK;
     if (!gradient || !temp || (n && (!tokens || !upstream))) return B200ALG_INVALID_ARGUMENT;
     if ((uintptr_t)gradient % ob || (uintptr_t)upstream % ib || (uintptr_t)tokens % dtype_bytes(token_dtype) || (uintptr_t)temp % 256)
         return B200ALG_MISALIGNED;

@@ -39,3 +39,11 @@ def test_nothing_is_written_behind_the_temp(accelerator, n, width, types):
     accelerator.CreateEmbeddingGradient()(None, tokens, upstream, out, whole[:ints])
     assert_within(out, *embedding_gradient(tokens, upstream, 1.0, 3, target))
     assert bool((whole[ints:] == 0x5A5A5A5A).all())
+
+
+@pytest.mark.parametrize("n, rows, width, accumulate", [(0, 5, 8, True), (0, 5, 8, False), (4, 0, 8, False), (4, 0, 8, True), (4, 5, 0, False), (0, 0, 0, True)])
+def test_an_empty_gradient_leaves_a_status(accelerator, n, rows, width, accumulate):
+    temp = torch.full((max(64, accelerator.ComputeEmbeddingGradientTempStorageSize(rows, width, n)),), -1, dtype=torch.int32, device="cuda")
+    tokens, upstream = torch.zeros(n, dtype=torch.int64, device="cuda"), torch.ones(n, width, device="cuda")
+    accelerator.CreateEmbeddingGradient(accumulate)(None, tokens, upstream, torch.empty(rows, width, device="cuda"), temp)
+    accelerator.CheckDeviceStatus(None, temp)
