@@ -176,6 +176,7 @@ struct BalanceShares {
 };
 
 struct BalanceResult {
+    TempHeader *hdr;
     double factor;  // coefficient * experts / choices
     float *loss;
     int *counts;
@@ -217,6 +218,7 @@ __device__ void finish_balance(const float *sums, const unsigned int *counts, in
         if (lane == 0) {
             *to.loss = (float)(sum * inverse * to.factor);
             to.counts[experts] = (int)valid;
+            to.hdr->wait_limit_hit = 0u;  // no wait can run out
         }
     }
 }
@@ -605,7 +607,7 @@ extern "C" int b200alg_balance_loss(void *stream, const void *logits, int64_t to
     BalanceShares shares;
     shares.sums = (float *)((char *)temp + sizeof(TempHeader));
     shares.counts = (unsigned int *)((char *)temp + sizeof(TempHeader) + round_up(kMostBalanceBlocks * experts * 4, 256));
-    const BalanceResult to{coefficient * experts / choices, loss, counts, probabilities};
+    const BalanceResult to{(TempHeader *)temp, coefficient * experts / choices, loss, counts, probabilities};
     const int group = router_group(experts, bytes, logits, logits_stride, logits, logits_stride, tokens);
     const int cluster = balance_cluster(tokens, experts, group >= 4);
     const size_t smem = balance_smem(experts, cluster);

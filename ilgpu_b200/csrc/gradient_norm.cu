@@ -245,11 +245,17 @@ template <int MOST, bool KEEP> __global__ void __launch_bounds__(kNormThreads) n
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-__global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(const double *partial, int count, float *norm) {
+// The norm, and the status word of the temp that the partial sums lie in: no wait of these kernels can run out.
+__device__ __forceinline__ void store_norm(float *norm, float whole, double *partial) {
+    *norm = whole;
+    (reinterpret_cast<TempHeader *>(partial) - 1)->wait_limit_hit = 0u;
+}
+
+__global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(double *partial, int count, float *norm) {
     grid_dependency_release();
     grid_dependency_wait();
     const float whole = norm_of(partial, count);
-    if (threadIdx.x == 0) *norm = whole;
+    if (threadIdx.x == 0) store_norm(norm, whole, partial);
 }
 
 template <typename TIn, typename TOut, typename Table> __device__ __forceinline__ void scale_part(const Part &part, const Table &t, float factor) {
@@ -296,7 +302,7 @@ __device__ __forceinline__ float factor_of(float norm, double max_norm) {
 // partial == NULL: by the norm that is there; else the norm comes from the blocks' sums, and the first block stores it.
 // (Every block adds them up itself, so that no launch stands between the two passes.)
 template <int MOST>
-__global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_constant__ ViewTable<MOST> t, const double *partial, int count, float *norm, double max_norm) {
+__global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_constant__ ViewTable<MOST> t, double *partial, int count, float *norm, double max_norm) {
     grid_dependency_release();
     Chunks<true, ViewTable<MOST>> at(t);
     bool more = at.enter();
@@ -306,7 +312,7 @@ __global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_consta
     float whole;
     if (partial) {
         whole = norm_of(partial, count);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *norm = whole;
+        if (blockIdx.x == 0 && threadIdx.x == 0) store_norm(norm, whole, partial);
     } else {
         whole = *norm;
     }
@@ -396,7 +402,7 @@ template <int MOST> static int run_partial(cudaStream_t s, const ViewLists &l, b
 }
 
 // By the norm that is there (partial == NULL), or by that of `sums` partial sums, which the first launch stores.
-template <int MOST> static int run_scale(cudaStream_t s, const ViewLists &l, const double *partial, int sums, float *norm, double max_norm) {
+template <int MOST> static int run_scale(cudaStream_t s, const ViewLists &l, double *partial, int sums, float *norm, double max_norm) {
     ViewTable<MOST> t;
     for (int64_t first = 0; first < l.count;) {
         first += fill_table(t, l.in, l.out, l.lengths, l.in_types, l.out_types, first, l.count);
@@ -422,8 +428,7 @@ template <int MOST> static int run_clip(cudaStream_t s, const ViewLists &l, floa
             B200ALG_CUDA_TRY(launch_with_table(max_norm >= 0.0 ? (const void *)norm_partial_kernel<MOST, true> : (const void *)norm_partial_kernel<MOST, false>,
                                                sums, s, arguments));
             if (max_norm >= 0.0) {
-                const double *from = partial;
-                void *scale_arguments[] = {&t, &from, &sums, &norm, &max_norm};
+                void *scale_arguments[] = {&t, &to, &sums, &norm, &max_norm};
                 B200ALG_CUDA_TRY(launch_with_table((const void *)scale_kernel<MOST>, sums, s, scale_arguments));
                 return B200ALG_OK;
             }
@@ -433,7 +438,7 @@ template <int MOST> static int run_clip(cudaStream_t s, const ViewLists &l, floa
         if (rc == B200ALG_OK && max_norm >= 0.0 && sums) rc = run_scale<MOST>(s, l, partial, sums, norm, max_norm);
         if (rc != B200ALG_OK || (max_norm >= 0.0 && sums)) return rc;
     }
-    B200ALG_CUDA_TRY(launch_dependent(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, (const double *)partial, sums, norm));
+    B200ALG_CUDA_TRY(launch_dependent(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, partial, sums, norm));
     return B200ALG_OK;
 }
 

@@ -317,7 +317,8 @@ int b200alg_balance_loss_gradient(void *stream, const void *logits, int64_t toke
 
 /* Device-side waits (decoupled look-back) are bounded; when one runs out the kernel
  * records it in `temp` and finishes.  This call copies that record back and
- * SYNCHRONISES `stream`: returns B200ALG_OK or B200ALG_WAIT_LIMIT. */
+ * SYNCHRONISES `stream`: returns B200ALG_OK or B200ALG_WAIT_LIMIT.  The norm and the balance
+ * loss wait for nothing; their calls leave B200ALG_OK. */
 int b200alg_device_status(void *stream, const void *temp);
 
 #ifdef __cplusplus

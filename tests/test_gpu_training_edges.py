@@ -47,3 +47,21 @@ def test_an_empty_gradient_leaves_a_status(accelerator, n, rows, width, accumula
     tokens, upstream = torch.zeros(n, dtype=torch.int64, device="cuda"), torch.ones(n, width, device="cuda")
     accelerator.CreateEmbeddingGradient(accumulate)(None, tokens, upstream, torch.empty(rows, width, device="cuda"), temp)
     accelerator.CheckDeviceStatus(None, temp)
+
+
+@pytest.mark.parametrize("lengths", [[], [0, 0], [1], [5, 70_000], [3] * 100, [3] * 1_500])
+def test_norm_and_clipping_leave_a_status(accelerator, lengths):
+    views, out = [torch.ones(n, device="cuda") for n in lengths], torch.empty(1, device="cuda")
+    temp = torch.empty(accelerator.ComputeGradientNormTempStorageSize(len(views)), dtype=torch.int32, device="cuda")
+    for call in (lambda: accelerator.CreateGradientNorm()(None, views, out, temp), lambda: accelerator.CreateGradientClip()(None, views, None, 1.0, out, temp)):
+        temp.fill_(-1)
+        call()
+        accelerator.CheckDeviceStatus(None, temp)
+
+
+@pytest.mark.parametrize("tokens, experts", [(0, 8), (5, 8), (1_000, 8), (3_000, 40), (20_000, 8)])
+def test_the_balance_loss_leaves_a_status(accelerator, tokens, experts):
+    temp = torch.full((accelerator.ComputeBalanceLossTempStorageSize(experts, tokens),), -1, dtype=torch.int32, device="cuda")
+    loss, counts, p = torch.empty(1, device="cuda"), torch.empty(experts + 1, dtype=torch.int32, device="cuda"), torch.empty(experts, device="cuda")
+    accelerator.CreateBalanceLoss(1.0)(None, torch.zeros(tokens, experts, device="cuda"), torch.zeros(tokens, 2, dtype=torch.int64, device="cuda"), None, loss, counts, p, temp)
+    accelerator.CheckDeviceStatus(None, temp)
