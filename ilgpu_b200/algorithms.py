@@ -855,6 +855,8 @@ class Accelerator:
                 raise ArgumentOutOfRangeException("logitsGradient")
             if logitsGradient.dtype != logits.dtype:
                 raise InvalidOperationException(f"logitsGradient: element type {logitsGradient.dtype}, expected {logits.dtype}")
+            if int(choices) > 2**31 - 1:
+                raise ArgumentOutOfRangeException("choices")
             self._check_device(logits, mask, counts, lossGradient, logitsGradient)
             with self.Bind():
                 B200AlgException.ThrowIfFailed(self.L.b200alg_balance_loss_gradient(

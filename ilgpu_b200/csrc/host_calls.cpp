@@ -557,7 +557,8 @@ PyObject *balance_loss_gradient(PyObject *, PyObject *const *a, Py_ssize_t count
     return guarded([&] {
         const int device = count == 10 ? device_of(a[0]) : -1;
         const double coefficient = PyFloat_AsDouble(a[1]);
-        const int choices = int_of(a[2]), accumulate = int_of(a[3]);
+        const int64_t choices = PyLong_AsLongLong(a[2]);
+        const int accumulate = int_of(a[3]);
         Matrix logits, gradient;
         View counts, loss_gradient;
         void *stream, *mask;

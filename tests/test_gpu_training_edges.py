@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import ilgpu_b200 as ib
+from ilgpu_b200 import _native as N
 
 from .training import TYPES, assert_within, embedding_gradient
 
@@ -65,3 +66,16 @@ def test_the_balance_loss_leaves_a_status(accelerator, tokens, experts):
     loss, counts, p = torch.empty(1, device="cuda"), torch.empty(experts + 1, dtype=torch.int32, device="cuda"), torch.empty(experts, device="cuda")
     accelerator.CreateBalanceLoss(1.0)(None, torch.zeros(tokens, experts, device="cuda"), torch.zeros(tokens, 2, dtype=torch.int64, device="cuda"), None, loss, counts, p, temp)
     accelerator.CheckDeviceStatus(None, temp)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("choices", [(1 << 32) + 2, (1 << 31) + 2, (1 << 64) + 2, 1_025, 0, -1, 2 - (1 << 32)])
+def test_choices_are_not_cut_to_a_word(monkeypatch, native, choices):
+    if not native:
+        monkeypatch.setattr(N, "_host", N._NoHostPath())
+    accelerator = ib.Accelerator(0)
+    logits, counts = torch.zeros(6, 8, device="cuda"), torch.tensor([3, 1, 1, 1, 2, 2, 1, 1, 6], dtype=torch.int32, device="cuda")
+    gradient = torch.full_like(logits, 7.0)
+    with pytest.raises((ib.ArgumentOutOfRangeException, ib.NotSupportedException, ib.B200AlgException)):
+        accelerator.CreateBalanceLossGradient(1.0, choices)(None, logits, None, counts, torch.ones(1, device="cuda"), gradient)
+    assert bool((gradient == 7.0).all())
