@@ -9,8 +9,8 @@
 //
 // The counts are taken as constants, as they have no derivative.
 //
-// One read of the logits (and one write of the gradient).  262144 tokens of 128 experts in bf16, 68 MB, take 25.1 us: 17.7 for the
-// probabilities, whose loads and exponentials 16 warps an SM do not hide altogether, 3.5 for the counts and 4.0 for the launch
+// One read of the logits (and one write of the gradient).  262144 tokens of 128 experts in bf16, 68 MB, take 25.7 us: 17.7 for the
+// probabilities, whose loads and exponentials 16 warps an SM do not hide altogether, 3.5 for the counts and 4.5 for the launch
 // that adds the blocks' shares up.  The gradient of 131072 tokens of 256 experts in float, 255 MB, takes 43.2 (5.9 TB/s).
 #include <math.h>
 #include <type_traits>
@@ -27,7 +27,11 @@ constexpr int kBalanceThreads = 512;  // (256, and so twice the shares to add up
 constexpr int kBalanceWarps = kBalanceThreads / 32;
 constexpr int kMostExperts = 1024;
 constexpr int kBalanceCluster = 8;  // blocks that add up in each other's shared memory
-constexpr int kMostBalanceBlocks = 148 * 3;
+constexpr int kMostBalanceBlocks = 148 * 2;  // (with 64 registers a thread or more no third one fits an SM)
+// Rows of a launch that a lane adds up.  With the lanes beside it and the block's warps a column's sum is 123 additions in 32
+// bits at most; blocks, clusters and launches go on in 64, so that the error does not grow with the tokens.  (Sums that
+// go on in 64 within a launch cost registers: 131072 tokens of 256 experts in float 33 us instead of 30.)
+constexpr int kLaneRows = 104;
 constexpr int kFinishThreads = 1024;
 constexpr int kIndexSlots = 2;        // indices of a row that a lane fetches ahead
 constexpr int kShareAhead = 8;      // blocks' shares that a thread has in flight
@@ -43,7 +47,7 @@ __host__ __device__ constexpr int padded_bins(int experts) { return (experts + 4
 constexpr int kGradientWarps = 8;
 // Shared memory of balance_kernel: counts, the warps' sums, and where one cluster is all a block's part of what it adds up.
 static size_t balance_smem(int64_t experts, int cluster) {
-    return (size_t)padded_bins((int)experts) * (1 + kBalanceWarps) * 4 + (cluster ? (size_t)ceil_div(experts, cluster) * 8 : 0);
+    return (size_t)padded_bins((int)experts) * (1 + kBalanceWarps) * 4 + (cluster ? (size_t)ceil_div(experts, cluster) * 12 : 0);
 }
 
 __device__ __forceinline__ float exp2_approximate(float x) {  // 2^x; below 2^-126 zero
@@ -171,8 +175,9 @@ __device__ __forceinline__ float inverse_of(float x) {
 
 // What the blocks found, in temp: sums of p by expert, and counts by expert with the tokens that count behind them.
 struct BalanceShares {
-    float *sums;           // [blocks][experts]
+    double *sums;          // [blocks][experts]
     unsigned int *counts;  // [blocks][experts + 1]
+    int add;               // to those of the launch before
 };
 
 struct BalanceResult {
@@ -192,7 +197,7 @@ __device__ __forceinline__ double sum_of_warp(double sum) {
 // The results from the sums and counts of all tokens, by the blocks of a cluster that are known to run: `sums` and
 // `counts` hold this block's columns [first, last) of the experts; `valid` tokens count.
 template <int THREADS>
-__device__ void finish_balance(const float *sums, const unsigned int *counts, int first, int last, unsigned int valid, int experts,
+__device__ void finish_balance(const double *sums, const unsigned int *counts, int first, int last, unsigned int valid, int experts,
                                const BalanceResult &to) {
     __shared__ double share[kBalanceCluster], part[THREADS / 32];
     cg::cluster_group cluster = cg::this_cluster();
@@ -324,22 +329,29 @@ balance_kernel(BalanceCall call, const T *__restrict__ logits, IndexView chosen,
             float p = sums[e];
 #pragma unroll
             for (int w = 1; w < kBalanceWarps; ++w) p += sums[w * experts + e];
-            if (alone) sums[e] = p;  // (this thread's own column)
-            else shares.sums[(int64_t)blockIdx.x * experts + e] = p;
+            if (alone) {
+                sums[e] = p;  // (this thread's own column)
+            } else {
+                double *share = shares.sums + (int64_t)blockIdx.x * experts + e;
+                *share = shares.add ? *share + p : p;
+            }
         }
-        if (!alone) shares.counts[(int64_t)blockIdx.x * (experts + 1) + e] = bins[e];
+        if (!alone) {
+            unsigned int *share = shares.counts + (int64_t)blockIdx.x * (experts + 1) + e;
+            *share = shares.add ? *share + bins[e] : bins[e];
+        }
     }
     if (!alone) return;
     // One cluster has all tokens: it adds up by columns and needs no other launch.
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), part = (experts + blocks - 1) / blocks, first = (int)cluster.block_rank() * part;
     const int last = first + part < experts ? first + part : experts;
-    float *all_sums = sums + kBalanceWarps * padded_bins(experts);                   // [part]
+    double *all_sums = reinterpret_cast<double *>(sums + kBalanceWarps * padded_bins(experts));  // [part]
     unsigned int *all_counts = reinterpret_cast<unsigned int *>(all_sums + part);    // [part]
     __shared__ unsigned int all_valid;
     cluster.sync();
     for (int e = first + threadIdx.x; e < last; e += kBalanceThreads) {
-        float p = 0.0f;
+        double p = 0.0;
         unsigned int n = 0u;
         for (int b = 0; b < blocks; ++b) {
             p += cluster.map_shared_rank(sums, b)[e];
@@ -356,11 +368,11 @@ balance_kernel(BalanceCall call, const T *__restrict__ logits, IndexView chosen,
     finish_balance<kBalanceThreads>(all_sums, all_counts, first, last, all_valid, experts, to);
 }
 
-// The shares of all blocks, by a cluster whose blocks take a part of the columns each (444 blocks' shares added up by
-// the threads of one block took it 60 us).
+// The shares of all blocks, by a cluster whose blocks take a part of the columns each.  (The threads of one block would
+// add up a few hundred shares one behind the other.)
 __global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(BalanceShares shares, int blocks, int experts, BalanceResult to) {
     constexpr int kMostColumns = kMostExperts / kBalanceCluster;
-    __shared__ float sums[kMostColumns], part[kFinishThreads];
+    __shared__ double sums[kMostColumns], part[kFinishThreads];
     __shared__ unsigned int counts[kMostColumns], part_counts[kFinishThreads], valid[kFinishThreads / 32];
     grid_dependency_release();
     const int columns = (experts + kBalanceCluster - 1) / kBalanceCluster, first = (int)blockIdx.x * columns;
@@ -373,15 +385,15 @@ __global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(BalanceS
     cg::this_cluster().sync();  // all its blocks run: they write to the first one's shared memory
     grid_dependency_wait();
     const unsigned int some_valid = threadIdx.x < blocks ? shares.counts[threadIdx.x * (experts + 1) + experts] : 0u;
-    float p = 0.0f;
+    double p = 0.0;
     unsigned int n = 0u;
     for (int b = ty; e < last && b < blocks; b += y * kShareAhead) {
-        float some[kShareAhead];
+        double some[kShareAhead];
         unsigned int count[kShareAhead];
 #pragma unroll
         for (int u = 0; u < kShareAhead; ++u) {
             const unsigned int at = b + u * y;  // (fewer than 2^20 values in all)
-            some[u] = at < blocks ? shares.sums[at * experts + e] : 0.0f;
+            some[u] = at < blocks ? shares.sums[at * experts + e] : 0.0;
             count[u] = at < blocks ? shares.counts[at * (experts + 1) + e] : 0u;
         }
 #pragma unroll
@@ -396,14 +408,13 @@ __global__ void __launch_bounds__(kFinishThreads) balance_finish_kernel(BalanceS
     if (lane == 0) valid[warp] = n;
     __syncthreads();
     for (int c = warp; c < columns; c += kFinishThreads / 32) {  // a warp adds up a column
-        p = 0.0f;
+        p = 0.0;
         n = 0u;
         for (int i = lane; i < y; i += 32) {
             p += part[i * x + c];
             n += part_counts[i * x + c];
         }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) p += __shfl_down_sync(0xffffffffu, p, d);
+        p = sum_of_warp(p);
         n = __reduce_add_sync(0xffffffffu, n);
         if (lane == 0) {
             sums[c] = p;
@@ -574,7 +585,7 @@ static int check_router(int64_t tokens, int64_t experts, int64_t choices, int64_
 
 static int64_t balance_temp_bytes(int64_t experts, int64_t tokens) {
     const int64_t blocks = balance_cluster(tokens, experts, false) ? 0 : kMostBalanceBlocks;
-    return sizeof(TempHeader) + round_up(blocks * experts * 4, 256) + round_up(blocks * (experts + 1) * 4, 256);
+    return sizeof(TempHeader) + round_up(blocks * experts * 8, 256) + round_up(blocks * (experts + 1) * 4, 256);
 }
 
 }  // namespace b200alg
@@ -605,8 +616,9 @@ extern "C" int b200alg_balance_loss(void *stream, const void *logits, int64_t to
     cudaStream_t s = (cudaStream_t)stream;
     int blocks = 0;
     BalanceShares shares;
-    shares.sums = (float *)((char *)temp + sizeof(TempHeader));
-    shares.counts = (unsigned int *)((char *)temp + sizeof(TempHeader) + round_up(kMostBalanceBlocks * experts * 4, 256));
+    shares.sums = (double *)((char *)temp + sizeof(TempHeader));
+    shares.counts = (unsigned int *)((char *)temp + sizeof(TempHeader) + round_up(kMostBalanceBlocks * experts * 8, 256));
+    shares.add = 0;
     const BalanceResult to{(TempHeader *)temp, coefficient * experts / choices, loss, counts, probabilities};
     const int group = router_group(experts, bytes, logits, logits_stride, logits, logits_stride, tokens);
     const int cluster = balance_cluster(tokens, experts, group >= 4);
@@ -618,16 +630,28 @@ extern "C" int b200alg_balance_loss(void *stream, const void *logits, int64_t to
         static ContextCache<int> cache;
         const int status = resident_blocks(kernel, kBalanceThreads, balance_smem(kMostExperts, 1), cache, &blocks);
         if (status != B200ALG_OK) return status;
+        int64_t most = tokens;  // of a launch
         if (cluster) {
             blocks = cluster;
         } else {
             const int64_t want = ceil_div(tokens, kBalanceWarps * S::ROWS * S::U);
             if (blocks > kMostBalanceBlocks) blocks = kMostBalanceBlocks;
             if (blocks > want) blocks = (int)want;
+            const int64_t rows = (int64_t)blocks * kBalanceWarps * S::ROWS;  // that the grid takes at a time
+            const int64_t rounds = ceil_div(tokens, rows);
+            most = ceil_div(rounds, ceil_div(rounds, kLaneRows)) * rows;  // as many rounds in each launch
         }
-        B200ALG_CUDA_TRY(launch_dependent_cluster(kernel, dim3(blocks), dim3(kBalanceThreads), smem, s, cluster ? cluster : 1,
-                                                  balance_call<S>(tokens, logits_stride, experts, choices, mask), (const T *)logits,
-                                                  IndexView{chosen, chosen_stride, chosen_dtype == B200ALG_I64}, shares, to, cluster != 0));
+        const int index_bytes = dtype_bytes(chosen_dtype);
+        int64_t first = 0;
+        do {
+            const int64_t some = tokens - first < most ? tokens - first : most;
+            B200ALG_CUDA_TRY(launch_dependent_cluster(
+                kernel, dim3(blocks), dim3(kBalanceThreads), smem, s, cluster ? cluster : 1,
+                balance_call<S>(some, logits_stride, experts, choices, mask ? (const char *)mask + first : nullptr), (const T *)logits + first * logits_stride,
+                IndexView{(const char *)chosen + first * chosen_stride * index_bytes, chosen_stride, chosen_dtype == B200ALG_I64}, shares, to, cluster != 0));
+            shares.add = 1;
+            first += most;
+        } while (first < tokens);
         return B200ALG_OK;
     });
     if (rc != B200ALG_OK || cluster) return rc;
