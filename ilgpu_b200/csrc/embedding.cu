@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupCall
     Columns<TIn, G, SHIFTED> in[kLookupItems];
     TOut *to[kLookupItems];
     int64_t column[kLookupItems];
+    float scale[kLookupItems];
 #pragma unroll
     for (int u = 0; u < kLookupItems; ++u) {
         const unsigned int q = base + u * kLookupThreads;
@@ -120,8 +121,10 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupCall
             const int64_t token = c.tokens[c.first + row];
             to[u] = out + (c.first + row) * c.out_stride;
             column[u] = column_of<SHIFTED, G>(to[u], q - row * groups.d);
-            if (token >= 0 && token < c.rows) in[u].load(table + token * c.row_stride + column[u], c.extent);
+            const bool there = token >= 0 && token < c.rows;
+            if (there) in[u].load(table + token * c.row_stride + column[u], c.extent);
             else in[u].clear();
+            scale[u] = there ? c.scale : 1.0f;  // (zeros whatever the scale)
         }
     }
 #pragma unroll
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupCall
         const Group<TIn, G> g = in[u].get();
         float x[G];
 #pragma unroll
-        for (int k = 0; k < G; ++k) x[k] = g.get(k) * c.scale;
+        for (int k = 0; k < G; ++k) x[k] = g.get(k) * scale[u];
         put_columns<SHIFTED>(to[u], column[u], c.width, x);
     }
 }

@@ -252,7 +252,7 @@ int b200alg_run_length_encode(void *stream, const void *data, int64_t n, int dty
  * rows, columns and tokens (B200ALG_TOO_LARGE). */
 
 /* out[i, 0..width) = scale * table[tokens[i], 0..width) for i in [0, n); zeros where
- * tokens[i] lies outside [0, rows). */
+ * tokens[i] lies outside [0, rows).  The scale is rounded to float, here and in the gradient. */
 int b200alg_embedding(void *stream, const void *table, int64_t rows, int64_t width, int64_t row_stride, int dtype,
                       const void *tokens, int64_t n, int64_t token_stride, int token_dtype, double scale, void *out,
                       int64_t out_stride, int out_dtype);

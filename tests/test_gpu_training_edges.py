@@ -79,3 +79,14 @@ def test_choices_are_not_cut_to_a_word(monkeypatch, native, choices):
     with pytest.raises((ib.ArgumentOutOfRangeException, ib.NotSupportedException, ib.B200AlgException)):
         accelerator.CreateBalanceLossGradient(1.0, choices)(None, logits, None, counts, torch.ones(1, device="cuda"), gradient)
     assert bool((gradient == 7.0).all())
+
+
+@pytest.mark.parametrize("types", ["bf16 bf16", "fp32 fp32", "fp32 fp16"])
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -2.0, 1e300])
+@pytest.mark.parametrize("width", [64, 33])
+def test_a_token_without_a_row_gets_zeros_whatever_the_scale(accelerator, width, scale, types):
+    source, target = (TYPES[t] for t in types.split())
+    out = torch.full((3, width), 7.0, dtype=target, device="cuda")
+    accelerator.CreateEmbedding()(None, torch.ones(4, width, dtype=source, device="cuda"), torch.tensor([-1, 2, 4], device="cuda"), out, scale)
+    assert not bool(out[[0, 2]].any()) and not bool(torch.signbit(out[[0, 2]]).any())
+    assert torch.equal(out[1].nan_to_num(7.0), torch.full((width,), scale, dtype=torch.float64, device="cuda").float().to(target).nan_to_num(7.0))
