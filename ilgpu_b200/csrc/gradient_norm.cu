@@ -258,7 +258,19 @@ __global__ void __launch_bounds__(kNormThreads) norm_finish_kernel(double *parti
     if (threadIdx.x == 0) store_norm(norm, whole, partial);
 }
 
-template <typename TIn, typename TOut, typename Table> __device__ __forceinline__ void scale_part(const Part &part, const Table &t, float factor) {
+// What the values are multiplied by, one behind the other.  A norm that is not finite leaves them as they are: it says so
+// itself.
+struct Factor {
+    float first, second;  // the second is 1 unless the factor as a whole is below float's normal numbers and would lose bits
+    __device__ __forceinline__ Factor(float norm, double max_norm) {
+        const double whole = norm <= FLT_MAX && (double)norm > max_norm ? max_norm / (double)norm : 1.0;
+        second = whole < (double)FLT_MIN ? FLT_MIN : 1.0f;
+        first = (float)(whole / (double)second);
+    }
+    __device__ __forceinline__ bool none() const { return first == 1.0f && second == 1.0f; }
+};
+
+template <typename TIn, typename TOut, typename Table> __device__ __forceinline__ void scale_part(const Part &part, const Table &t, const Factor &factor) {
     constexpr int G = kGroupBytes / (int)sizeof(TIn);
     constexpr unsigned int kBoundary = G * sizeof(TOut);
     const int64_t length = t.length[part.view];
@@ -272,7 +284,11 @@ template <typename TIn, typename TOut, typename Table> __device__ __forceinline_
         g.w[0] = part.w[u].x, g.w[1] = part.w[u].y, g.w[2] = part.w[u].z, g.w[3] = part.w[u].w;
         float x[G];
 #pragma unroll
-        for (int k = 0; k < G; ++k) x[k] = g.get(k) * factor;
+        for (int k = 0; k < G; ++k) x[k] = g.get(k) * factor.first;
+        if (factor.second != 1.0f) {
+#pragma unroll
+            for (int k = 0; k < G; ++k) x[k] *= factor.second;
+        }
         if (first >= 0 && first + G <= length && (uintptr_t)to % kBoundary == 0) {
             Group<TOut, G> y;
             y.set(x);
@@ -285,17 +301,12 @@ template <typename TIn, typename TOut, typename Table> __device__ __forceinline_
     }
 }
 
-template <typename TIn, typename Table> __device__ __forceinline__ void scale_part_from(const Part &part, const Table &t, float factor) {
+template <typename TIn, typename Table> __device__ __forceinline__ void scale_part_from(const Part &part, const Table &t, const Factor &factor) {
     switch (t.out_type[part.view]) {
     case B200ALG_F32: scale_part<TIn, float>(part, t, factor); break;
     case B200ALG_F16: scale_part<TIn, __half>(part, t, factor); break;
     default: scale_part<TIn, __nv_bfloat16>(part, t, factor);
     }
-}
-
-// What the values are multiplied by.  A norm that is not finite leaves them as they are: it says so itself.
-__device__ __forceinline__ float factor_of(float norm, double max_norm) {
-    return norm <= FLT_MAX && (double)norm > max_norm ? (float)(max_norm / (double)norm) : 1.0f;
 }
 
 // Backwards, and each block what it has read for the norm: what was read last may still be in the cache.
@@ -316,9 +327,9 @@ __global__ void __launch_bounds__(kNormThreads) scale_kernel(const __grid_consta
     } else {
         whole = *norm;
     }
-    const float factor = factor_of(whole, max_norm);
-    if (factor == 1.0f && t.in_place) return;
-    auto changes = [&](int view) { return factor != 1.0f || t.in[view] != t.out[view]; };  // else it is neither read nor written
+    const Factor factor(whole, max_norm);
+    if (factor.none() && t.in_place) return;
+    auto changes = [&](int view) { return !factor.none() || t.in[view] != t.out[view]; };  // else it is neither read nor written
     while (more) {
         const Part part = next;
         more = at.next();

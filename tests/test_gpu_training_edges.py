@@ -6,7 +6,7 @@ import torch
 import ilgpu_b200 as ib
 from ilgpu_b200 import _native as N
 
-from .training import TYPES, assert_within, embedding_gradient
+from .training import TYPES, assert_within, clipped, embedding_gradient
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,27 @@ def test_a_token_without_a_row_gets_zeros_whatever_the_scale(accelerator, width,
     accelerator.CreateEmbedding()(None, torch.ones(4, width, dtype=source, device="cuda"), torch.tensor([-1, 2, 4], device="cuda"), out, scale)
     assert not bool(out[[0, 2]].any()) and not bool(torch.signbit(out[[0, 2]]).any())
     assert torch.equal(out[1].nan_to_num(7.0), torch.full((width,), scale, dtype=torch.float64, device="cuda").float().to(target).nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("types", ["fp32 fp32", "fp32 bf16", "bf16 fp32", "bf16 bf16"])
+@pytest.mark.parametrize("given, max_norm", [(3e38, 1.0), (3e38, 3e-3), (3e38, 1e-7), (1e38, 1e-20), (1e20, 1e-19), (1e30, 1e-37), (3e38, 0.0), (1e-30, 1e-44), (2e37, 0.2)])
+def test_factors_below_the_normal_numbers(accelerator, given, max_norm, types):
+    """max_norm / norm may be a number that float holds with few bits, or not at all, while the products are ordinary numbers."""
+    source, target = (TYPES[t] for t in types.split())
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    sizes = torch.rand(5_001, generator=gen, device="cuda").mul_(80.0).sub_(80.0).exp_()  # all the way down to subnormal products
+    view = (torch.randn(5_001, generator=gen, device="cuda").clamp_(-1.0, 1.0) * given * sizes).to(source)
+    before, norm = view.clone(), torch.tensor([given], device="cuda")
+    out = torch.empty_like(view, dtype=target)
+    accelerator.CreateGradientScale()(None, [view], [out], max_norm, norm)
+    assert_within(out, *clipped(before, float(norm), max_norm, target))
+    if source == target:
+        accelerator.CreateGradientScale()(None, [view], None, max_norm, norm)
+        assert torch.equal(view, out)
+
+
+def test_clipping_of_the_largest_gradients(accelerator):
+    view, norm = torch.tensor([1e38, -2e38, 3e37, 1.0, 0.0], device="cuda"), torch.empty(1, device="cuda")
+    before, temp = view.clone(), torch.empty(accelerator.ComputeGradientNormTempStorageSize(1), dtype=torch.int32, device="cuda")
+    accelerator.CreateGradientClip()(None, [view], None, 1.0, norm, temp)
+    assert_within(view, *clipped(before, float(norm), 1.0, torch.float32))
