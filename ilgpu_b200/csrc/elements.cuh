@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "fast_divide.cuh"
 
 #include <cuda_bf16.h>
 
@@ -29,19 +30,6 @@ inline bool matrix_ok(int64_t rows, int64_t width, int64_t row_stride) {
 }
 
 inline bool index_dtype(int dt) { return dt == B200ALG_I32 || dt == B200ALG_I64; }
-
-// Division of q < 2^31 by a number that a launch has in common: q / d = (high word of q * m + q) >> s.
-struct FastDivide {
-    unsigned int m, s, d;
-    FastDivide() = default;
-    explicit FastDivide(unsigned int divisor) : d(divisor) {
-        for (s = 0; s < 32 && (1ull << s) < d; ++s) {}
-        m = (unsigned int)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
-    }
-#ifdef __CUDACC__
-    __device__ __forceinline__ unsigned int operator()(unsigned int q) const { return (__umulhi(q, m) + q) >> s; }
-#endif
-};
 
 #ifdef __CUDACC__
 
