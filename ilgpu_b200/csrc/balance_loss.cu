@@ -11,7 +11,7 @@
 //
 // One read of the logits (and one write of the gradient).  262144 tokens of 128 experts in bf16, 68 MB, take 25.7 us: 17.7 for the
 // probabilities, whose loads and exponentials 16 warps an SM do not hide altogether, 3.5 for the counts and 4.5 for the launch
-// that adds the blocks' shares up.  The gradient of 131072 tokens of 256 experts in float, 255 MB, takes 43.2 (5.9 TB/s).
+// that adds the blocks' shares up.  The gradient of 131072 tokens of 256 experts in float, 255 MB, takes 42.2 (6.0 TB/s).
 #include <math.h>
 #include <type_traits>
 
@@ -555,8 +555,8 @@ template <typename S> static BalanceCall balance_call(int64_t tokens, int64_t lo
 }
 
 // Blocks of a call: one for a few rows, then a cluster of them, and from where one is slower than two launches (0) as
-// many as there is work for.  In bf16 64 experts, us, cluster / two launches: 2048 tokens 6.6 / 7.2, 4096 8.9 / 7.6; rows
-// that do not lie on boundaries take longer: 1576 tokens of 99 experts in float 13.7 / 8.
+// many as there is work for.  In bf16 64 experts, us, cluster / two launches: 128 tokens 5.7 / 7.3, 2048 6.9 / 8.5, 2437
+// 7.7 / 8.4; rows that do not lie on boundaries take longer: of 99 experts in float 330 tokens 5.3 / 7.4, 1323 7.9 / 7.5.
 static int balance_cluster(int64_t tokens, int64_t experts, bool long_groups) {
     const int64_t cells = tokens * experts;
     return cells <= 4096 ? 1 : cells <= (long_groups ? 1 << 17 : 1 << 15) ? kBalanceCluster : 0;

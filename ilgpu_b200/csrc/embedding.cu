@@ -450,9 +450,11 @@ __global__ void __launch_bounds__(kGradientThreads) gradient_join_kernel(Gradien
 // ---- gradient of few tokens, in one launch ----
 // A block of a position looks all tokens over: if its token stands in front of it, another block has its row; else it
 // lists the positions that name the row and adds them up, in y parts that are joined in order.  What clears does so with
-// the bits of its own rows, from all tokens as well.  (Sorting them would take one block 13 us and the launches around it
-// 5, whatever the table.)
-constexpr int64_t kFewTokens = 512, kMostFewTokens = 1024;  // the latter where a row is one part of a block: 840 of 64 floats 10 us, by a sort 19
+// the bits of its own rows, from all tokens as well.  us, this way / by a sort, into 500 rows and into 32000:
+//   257 tokens of   64 floats   4.8 / 14.0    6.1 / 15.2        1024 tokens of   64 floats  10.2 / 14.9   11.0 / 17.0
+//   512 tokens of 4096 bf16    15.4 / 15.9   78.0 / 86.0         640 tokens of 4096 bf16    19.3 / 16.8   79.1 / 86.5
+//   512 tokens of 1357 bf16    13.1 / 16.4   40.2 / 42.5         640 tokens of 1357 bf16    16.7 / 16.8   44.4 / 42.8
+constexpr int64_t kFewTokens = 512, kMostFewTokens = 1024;  // the latter where a row is one part of a block
 
 template <typename TIn, typename TOut, int G, bool SHIFTED>
 __global__ void __launch_bounds__(kGradientThreads)

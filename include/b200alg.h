@@ -244,7 +244,9 @@ int b200alg_run_length_encode(void *stream, const void *data, int64_t n, int dty
  * histogram.  No counterpart in the reference.
  *
  * Element types are F32, F16 and BF16; sums are held in 32 bits or more, in an order that
- * depends on sizes only, and results are rounded once.  Token and expert indices are I32 or
+ * depends on nothing but sizes, types, strides, how the buffers lie to boundaries of 32 bytes
+ * and the GPU's number of SMs (equal calls over the same buffers give equal bits, data that was
+ * moved may not), and results are rounded once.  Token and expert indices are I32 or
  * I64.  Matrices are row-major with rows `*_stride` elements apart; what lies between the
  * width of a row and the next row is not written, and what it holds does not matter (a load
  * may take in bytes beside a row that share an aligned 16 bytes with it).  Outputs overlap no input
@@ -298,7 +300,8 @@ int b200alg_gradient_clip(void *stream, const void *const *views, void *const *o
  * p_te, loss[0] = coefficient * experts * sum over e of c_e / (T' choices) * P_e.  Only
  * tokens with mask[t] != 0 (bytes; NULL: all) count, T' of them; the others' logits and
  * choices are not read.  A row of nothing but -inf has p = 0.  counts[0..experts) = c_e,
- * counts[experts] = T' (int32), probabilities[e] = P_e (float); T' = 0 gives zeros. */
+ * counts[experts] = T' (int32), probabilities[e] = P_e (float); T' = 0 gives zeros.
+ * tokens * choices is at most 2^31 - 1, as the counts are (B200ALG_TOO_LARGE). */
 int b200alg_balance_loss_temp_bytes(int64_t experts, int64_t tokens, int64_t *out_bytes);
 int b200alg_balance_loss(void *stream, const void *logits, int64_t tokens, int64_t experts, int64_t logits_stride,
                          int dtype, const void *chosen, int64_t choices, int64_t chosen_stride, int chosen_dtype,
