@@ -7,7 +7,6 @@
 #include <type_traits>
 
 #include "elements.cuh"
-#include "sort_common.cuh"
 
 namespace b200alg {
 
@@ -642,7 +641,7 @@ static int run_gradient(cudaStream_t s, GradientCall c, const IndexView &tokens,
     if (named)
         B200ALG_CUDA_TRY(launch_dependent(gradient_forget_kernel, some(ceil_div(L.named_words, 256)), dim3(256), 0, s, (uint4 *)named, L.named_words));
     B200ALG_CUDA_TRY(launch_dependent(gradient_keys_kernel, some(ceil_div(c.n, 256 * 2)), dim3(256), 0, s, tokens, c.n, c.rows, keys, named));
-    const int rc = sort_with_positions(s, keys, positions, c.n, temp, L.sort_bytes);
+    const int rc = b200alg_radix_sort_pairs_sequence(s, keys, positions, c.n, B200ALG_U32, B200ALG_U32, B200ALG_SORT_ASCENDING, temp, L.sort_bytes);
     if (rc != B200ALG_OK) return rc;
     const size_t smem = (size_t)c.y * (2 * c.tile + 3) * 4;  // (33 KB at most)
     B200ALG_CUDA_TRY(launch_dependent(gradient_sum_kernel<TIn, TOut, G, SHIFTED>, dim3((unsigned)c.sum_blocks), dim3(kGradientThreads), smem, s, c,

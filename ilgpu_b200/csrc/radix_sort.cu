@@ -1387,11 +1387,6 @@ static int sort_common(void *stream, const SortCall &call, int key_dtype, int va
     return B200ALG_UNSUPPORTED;
 }
 
-int sort_with_positions(void *stream, unsigned int *keys, unsigned int *positions, int64_t n, void *temp, int64_t temp_bytes) {
-    const SortCall call{keys, keys, positions, positions, 1, n, nullptr, kSeqInteger, false};
-    return sort_common(stream, call, B200ALG_U32, 4, B200ALG_SORT_ASCENDING, temp, temp_bytes);
-}
-
 }  // namespace b200alg
 
 using namespace b200alg;

@@ -109,7 +109,4 @@ int sample_sort(cudaStream_t s, const SortCall &call, int key_bytes, int value_b
 int resident_sort(cudaStream_t s, const SortCall &call, int key_bytes, int value_bytes, uint64_t xor_neg, uint64_t xor_pos, void *temp,
                   int64_t temp_bytes, bool *taken);
 
-// b200alg_radix_sort_pairs_sequence for unsigned keys with their positions (radix_sort.cu).
-int sort_with_positions(void *stream, unsigned int *keys, unsigned int *positions, int64_t n, void *temp, int64_t temp_bytes);
-
 }  // namespace b200alg
