@@ -162,7 +162,7 @@ static int run_lookup(cudaStream_t s, const void *table, int64_t rows, int64_t w
 // table, are known from a byte each and cleared by other blocks of the last launch, beside the join, which waits more than it
 // moves.  (Beside the sums the join stands alone at the end: 75.8 us instead of 70.3 for 16384 tokens.  The sort, too, is
 // independent of the clearing, but a launch that passes it by without a wait is not promised to find the bytes written.)
-// Memory is the bound: 131072 rows of 4096 bf16 into 128000 rows of float take 526 us, 3.2 GB at 5.9 TB/s; 16384 of 2048
+// Memory is the bound: 131072 rows of 4096 bf16 into 128000 rows of float take 506 us, 3.1 GB at 6.2 TB/s; 16384 of 2048
 // into 32000 take 70, some 15 of them for keys and sort in front of 330 MB.
 constexpr int kGradientThreads = 256;
 constexpr int kAhead = 8;      // rows, or shares, that a thread has in flight

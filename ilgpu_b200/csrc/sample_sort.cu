@@ -164,7 +164,6 @@ sample_sort_kernel(SampleSort<K, V> a) {
     b.shared = local_shared(smem);
     local_clear(b.shared);
     grid_dependency_wait();
-    grid_dependency_release();
     b.n = (unsigned int)effective_n(a.io);
     const unsigned int share = (b.n + blocks - 1) / blocks;
     b.lo = blockIdx.x * share < b.n ? blockIdx.x * share : b.n;

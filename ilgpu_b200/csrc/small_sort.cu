@@ -78,7 +78,6 @@ resident_sort_kernel(SortBuffers<K, V> io, KeyXform<K> xf, TempHeader *hdr, unsi
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_dependency_wait();
-    grid_dependency_release();
     const int64_t n = effective_n(io);
     const int64_t base = (int64_t)blockIdx.x * tile;
     const int valid = (int)(n - base < 0 ? 0 : (n - base < tile ? n - base : tile));
@@ -387,7 +386,6 @@ block_sort_kernel(SortBuffers<K, V> io, KeyXform<K> xf, TempHeader *hdr, int ite
     const LocalShared shared = local_shared(smem);
     local_clear(shared);
     grid_dependency_wait();
-    grid_dependency_release();
     const int count = (int)effective_n(io);
     if (tid == 0) hdr->wait_limit_hit = 0u;
 
